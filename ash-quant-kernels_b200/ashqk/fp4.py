@@ -1,0 +1,163 @@
+"""Microscaled 4-bit floating point: MXFP4 and NVFP4 tensors, their quantiser and their products.
+
+Beside the AWQ integers (``quantize_awq``, ``w4a16_linear``), whose weights are 4-bit and whose products
+are 16-bit, these hold both operands in a form that the B200 tensor core multiplies as it is.
+
+An element is E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives); a block of a row's columns shares a scale:
+
+    "mxfp4"  32 columns  scale 2^(floor(log2 amax) - 2), held as E8M0
+    "nvfp4"  16 columns  scale E4M3(min(448, amax / (6 g))) times the tensor's global scale g
+
+An element is its value over the scale, rounded to nearest even and held to +-6. All of it runs on CUDA
+tensors only, on the current stream, allocates through PyTorch and can be captured in a CUDA graph.
+No reference counterpart: the reference multiplies 4-bit weights in 16 bits.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _ext
+
+FP4_FORMATS = ("mxfp4", "nvfp4")
+_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_CODE = {"mxfp4": 0, "nvfp4": 1}
+_E4M3_MAX, _E2M1_MAX = 448.0, 6.0
+
+_op_cache: dict = {}
+
+
+def _op(name: str):
+    op = _op_cache.get(name)
+    if op is None:
+        op = _op_cache[name] = getattr(_ext.ops(), name).default
+    return op
+
+
+def _format(fmt: str) -> int:
+    code = _CODE.get(fmt)
+    assert code is not None, f"format must be one of {FP4_FORMATS}, got {fmt!r}"
+    return code
+
+
+def _check_global_scale(fmt: str, g: float) -> None:
+    assert g == 1.0 if fmt == "mxfp4" else 1e-18 <= g <= 1e18, \
+        f"global_scale {g} out of range (1 for mxfp4, 1e-18 .. 1e18 for nvfp4)"
+
+
+class FP4Tensor:
+    """A matrix [rows, K] in microscaled 4-bit form: what ``quantize_fp4`` returns and the products take.
+
+    codes   uint8 [rows, ceil(K / 32) * 16]: two elements to a byte, the even column in the low four
+            bits; columns from K on are zero; rows may be strided by a multiple of 16 bytes
+    scales  uint8 [ceil(rows / 128), ceil(blocks / 4), 32, 4, 4], contiguous, ``blocks`` = K rounded up to 32
+            over the block size: the scale of (row, block) lies at
+            [row // 128, block // 4, row % 32, row // 32 % 4, block % 4]. Rows and blocks beyond the matrix
+            are padding: blocks 0, rows anything.
+    """
+
+    __slots__ = ("codes", "scales", "shape", "format", "global_scale")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, format: str = "mxfp4", global_scale: float = 1.0):
+        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+        self.format, self.global_scale = format, global_scale
+
+    @staticmethod
+    def from_rowmajor(codes: torch.Tensor, scales: torch.Tensor, format: str = "mxfp4", global_scale: float = 1.0) -> "FP4Tensor":
+        """From a checkpoint's plain layout: codes uint8 [rows, K / 2], scales [rows, K / block] (uint8, or float8
+        of the format's kind). K is a multiple of the block."""
+        _format(format)
+        _check_global_scale(format, global_scale)
+        block = _BLOCK[format]
+        assert codes.dtype == torch.uint8 and codes.dim() == 2 and scales.dim() == 2
+        rows, k = codes.shape[0], 2 * codes.shape[1]
+        if scales.dtype != torch.uint8:
+            assert scales.dtype == (torch.float8_e8m0fnu if format == "mxfp4" else torch.float8_e4m3fn)
+            scales = scales.view(torch.uint8)
+        assert k % block == 0 and k > 0 and scales.shape == (rows, k // block), \
+            f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not {format} of one matrix"
+        kp = -(-k // 32) * 32
+        blocks = kp // block
+        codes = torch.nn.functional.pad(codes, (0, (kp - k) // 2)).contiguous()
+        tiles, cols = -(-rows // 128), -(-blocks // 4)
+        full = scales.new_zeros(tiles * 128, cols * 4)
+        full[:rows, : k // block] = scales
+        tiled = full.view(tiles, 4, 32, cols, 4).permute(0, 3, 2, 1, 4).contiguous()
+        return FP4Tensor(codes, tiled, (rows, k), format, global_scale)
+
+    def scales_rowmajor(self) -> torch.Tensor:
+        """The scale bytes as uint8 [rows, ceil(K / block)]."""
+        tiles, cols = self.scales.shape[:2]
+        flat = self.scales.permute(0, 3, 2, 1, 4).reshape(tiles * 128, cols * 4)
+        return flat[: self.shape[0], : -(-self.shape[1] // _BLOCK[self.format])].contiguous()
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __repr__(self) -> str:
+        return f"FP4Tensor({self.shape}, {self.format!r}, global_scale={self.global_scale}, device={self.device})"
+
+
+def fp4_global_scale(x: torch.Tensor) -> float:
+    """The NVFP4 global scale that maps the largest magnitude of x onto the largest value of the format
+    (amax / (448 * 6)); 1 for a tensor of zeros. Copies one number to the host."""
+    amax = float(x.detach().abs().amax()) if x.numel() else 0.0
+    assert math.isfinite(amax), "x holds an infinity or a NaN"
+    g = float(torch.tensor(amax / (_E4M3_MAX * _E2M1_MAX), dtype=torch.float32))
+    return g if g >= 1e-18 else 1.0
+
+
+def _quantize(x: torch.Tensor, fmt: str, global_scale: float, gated: bool) -> FP4Tensor:
+    code = _format(fmt)
+    _check_global_scale(fmt, global_scale)
+    k = x.shape[-1]
+    if gated:
+        assert k % 2 == 0, "gate and up are the two halves of the last dimension"
+        k //= 2
+    codes, scales = _op("quantize_fp4")(x, code, global_scale, gated)
+    return FP4Tensor(codes, scales, (codes.shape[0], k), fmt, global_scale)
+
+
+def quantize_fp4(x: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
+    """x [..., K] (fp16, bf16 or fp32) -> FP4Tensor of shape (rows, K); any K, strided rows as they are.
+
+    ``global_scale`` belongs to "nvfp4" (see ``fp4_global_scale``); a block with an infinity or a NaN
+    reads back as NaN.
+    """
+    return _quantize(x, format, global_scale, False)
+
+
+def silu_mul_quantize_fp4(gate_up: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
+    """gate_up [..., 2 K] -> FP4Tensor of silu(gate) * up, gate and up the two halves of the last dimension.
+
+    The activation is computed in fp32 and rounded once, to the format: one pass over gate_up.
+    """
+    return _quantize(gate_up, format, global_scale, True)
+
+
+def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of q, [rows, K] in fp16, bf16 or fp32."""
+    return _op("dequantize_fp4")(q.codes, q.scales, q.shape[1], _format(q.format), q.global_scale, dtype)
+
+
+def fp4_matmul(a: FP4Tensor, b: FP4Tensor, dtype: torch.dtype = torch.float16) -> torch.Tensor:
+    """a [M, K] @ b [N, K]^T in fp32, rounded to fp16 or bf16. Both operands have the same format."""
+    assert a.format == b.format, f"operands of two formats: {a.format}, {b.format}"
+    assert a.shape[1] == b.shape[1], f"K differs: {a.shape}, {b.shape}"
+    return _op("fp4_matmul")(a.codes, a.scales, b.codes, b.scales, a.shape[1], _format(a.format),
+                             a.global_scale * b.global_scale, dtype)
+
+
+def w4a4_linear(x: torch.Tensor, weight: FP4Tensor, *, global_scale: float = 1.0, gated: bool = False) -> torch.Tensor:
+    """y = Q(x) @ weight^T: x [..., K] fp16 or bf16 is quantised to the weights' format on the way; y [..., N]
+    has x's type.
+
+    ``gated``: x is [..., 2 K] and silu(x[..., :K]) * x[..., K:] takes its place (an MLP's down
+    projection). ``global_scale`` is x's, for "nvfp4".
+    """
+    _check_global_scale(weight.format, global_scale)
+    return _op("w4a4_linear")(x, weight.codes, weight.scales, weight.shape[1], _format(weight.format), global_scale,
+                              weight.global_scale, gated)

@@ -1,0 +1,50 @@
+// W4A4 linear layer: x in 16 bits, quantised on the way into the product with 4-bit weights.
+#include "fp4.cuh"
+
+namespace ashqk {
+
+int dtype_size(int dtype);
+int check_fp4_operand(const void* codes, int64_t codes_ld, const void* scales, int K);
+bool fp4_global_scale_ok(int format, float gs);
+int quantize_fp4(const void* x, int64_t x_ld, int dtype, bool gated, void* codes, int64_t codes_ld, void* scales, int M,
+                 int K, int format, float gs, bool early, cudaStream_t stream);
+
+namespace {
+
+// Q(x) in the workspace: scales first (a multiple of 512 bytes), then codes.
+void workspace_layout(int M, int K, int format, size_t* codes_offset, size_t* bytes) {
+  *codes_offset = static_cast<size_t>(ceil_div64(M, kFp4TileRows) * fp4_scale_tiles(K, format) * kFp4TileBytes);
+  *bytes = *codes_offset + static_cast<size_t>(M) * (fp4_padded_k(K) / 2);
+}
+
+}  // namespace
+}  // namespace ashqk
+
+using namespace ashqk;
+
+extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes) {
+  if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  size_t offset;
+  workspace_layout(M, K, format, &offset, bytes);
+  return ASHQK_OK;
+}
+
+extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gated, float x_scale, const void* w_codes,
+                                 int64_t w_ld, const void* w_scales, float w_scale, void* y, int64_t y_ld, int M, int N,
+                                 int K, int format, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!x || !y || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(x, 2) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (x_ld < static_cast<int64_t>(K) * (gated ? 2 : 1) || y_ld < N) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!fp4_global_scale_ok(format, x_scale) || !fp4_global_scale_ok(format, w_scale)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (const int rc = check_fp4_operand(w_codes, w_ld, w_scales, K)) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  size_t offset, bytes;
+  workspace_layout(M, K, format, &offset, &bytes);
+  if (!workspace || workspace_bytes < bytes || !aligned(workspace, 16)) return ASHQK_ERR_WORKSPACE;
+  uint8_t* scales = static_cast<uint8_t*>(workspace);
+  uint8_t* codes = scales + offset;
+  const int64_t ld = fp4_padded_k(K) / 2;
+  if (const int rc = quantize_fp4(x, x_ld, dtype, gated != 0, codes, ld, scales, M, K, format, x_scale, true, st)) return rc;
+  return ashqk_fp4_matmul(codes, ld, scales, w_codes, w_ld, w_scales, y, y_ld, dtype, M, N, K, format, x_scale * w_scale,
+                          stream);
+}

@@ -13,7 +13,9 @@
 
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
+#include <vector>
 
 #include "ashqk_b200.h"
 
@@ -175,6 +177,141 @@ at::Tensor dequantize_awq(const at::Tensor& qw_in, const at::Tensor& qz_in, cons
   return w;
 }
 
+// ---- microscaled 4-bit floating point ----------------------------------------------------------
+
+int fp4_dtype(at::ScalarType t) {
+  return t == at::kHalf ? ASHQK_F16 : t == at::kBFloat16 ? ASHQK_BF16 : t == at::kFloat ? ASHQK_F32 : -1;
+}
+
+// A tensor with rows of `cols` values as a matrix the kernels take: unit column stride, rows that do not
+// overlap. A copy only where the caller's layout is neither.
+struct Rows {
+  at::Tensor t;
+  int64_t rows, ld;
+};
+
+Rows as_rows(const at::Tensor& x, int64_t cols) {
+  Rows r;
+  r.t = x.dim() == 2 ? x : x.reshape({cols ? x.numel() / cols : 0, cols});
+  if (r.t.stride(1) != 1 || (r.t.size(0) > 1 && r.t.stride(0) < cols)) r.t = r.t.contiguous();
+  r.rows = r.t.size(0);
+  r.ld = r.rows > 1 ? r.t.stride(0) : cols;
+  TORCH_CHECK(r.rows <= INT32_MAX, "ashqk: problem too large");
+  return r;
+}
+
+void check_no_grad(const at::Tensor& x, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "ashqk.", what,
+              " has no gradient: call it under torch.no_grad() or with x.detach()");
+}
+
+void check_fp4(const at::Tensor& codes, const at::Tensor& scales, int64_t K, int64_t format, const at::Device& dev) {
+  TORCH_CHECK(K > 0 && K <= (1 << 30), "ashqk: K out of range");
+  TORCH_CHECK(codes.device() == dev && scales.device() == dev, "ashqk: all tensors must be on the same device");
+  TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 2 && codes.size(1) == (K + 31) / 32 * 16 &&
+                  codes.stride(1) == 1,
+              "ashqk: codes must be uint8 [rows, ceil(K / 32) * 16] with unit column stride");
+  TORCH_CHECK(codes.size(0) <= INT32_MAX, "ashqk: problem too large");
+  int64_t ld = 0, bytes = 0;
+  TORCH_CHECK(ashqk_fp4_sizes(static_cast<int>(codes.size(0)), static_cast<int>(K), static_cast<int>(format), &ld, &bytes) == ASHQK_OK,
+              "ashqk: unknown 4-bit format ", format);
+  TORCH_CHECK(scales.scalar_type() == at::kByte && scales.is_contiguous() && scales.numel() == bytes,
+              "ashqk: scales must be contiguous uint8 [ceil(rows / 128), ceil(blocks / 4), 32, 4, 4]");
+}
+
+int64_t codes_ld(const at::Tensor& codes) { return codes.size(0) > 1 ? codes.stride(0) : codes.size(1); }
+
+at::Tensor empty_scales(int64_t rows, int64_t K, int64_t format, const at::TensorOptions& opt) {
+  const int64_t blocks = (K + 31) / 32 * (format == ASHQK_MXFP4 ? 1 : 2);
+  return at::empty({(rows + 127) / 128, (blocks + 3) / 4, 32, 4, 4}, opt.dtype(at::kByte));
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_fp4(const at::Tensor& x, int64_t format, double global_scale, bool gated) {
+  TORCH_CHECK(x.is_cuda(), "ashqk: x must be a CUDA tensor");
+  const int dtype = fp4_dtype(x.scalar_type());
+  TORCH_CHECK(dtype >= 0 && x.dim() >= 1, "ashqk: x must be a float16, bfloat16 or float32 tensor of at least one dimension");
+  check_no_grad(x, "quantize_fp4");
+  TORCH_CHECK(format == ASHQK_MXFP4 || format == ASHQK_NVFP4, "ashqk: unknown 4-bit format ", format);
+  const int64_t cols = x.size(-1), K = gated ? cols / 2 : cols;
+  TORCH_CHECK(K > 0 && K <= (1 << 30) && (!gated || cols % 2 == 0), "ashqk: x needs columns (an even number when gated)");
+  c10::cuda::CUDAGuard guard(x.device());
+  const Rows r = as_rows(x, cols);
+  at::Tensor codes = at::empty({r.rows, (K + 31) / 32 * 16}, x.options().dtype(at::kByte));
+  at::Tensor scales = empty_scales(r.rows, K, format, x.options());
+  if (r.rows == 0) return {codes, scales};
+  check_rc(ashqk_quantize_fp4(r.t.data_ptr(), r.ld, dtype, gated, codes.data_ptr(), codes.size(1), scales.data_ptr(),
+                              static_cast<int>(r.rows), static_cast<int>(K), static_cast<int>(format),
+                              static_cast<float>(global_scale), c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+           "quantize_fp4");
+  return {codes, scales};
+}
+
+at::Tensor dequantize_fp4(const at::Tensor& codes, const at::Tensor& scales, int64_t K, int64_t format,
+                          double global_scale, at::ScalarType dtype) {
+  TORCH_CHECK(codes.is_cuda(), "ashqk: codes must be a CUDA tensor");
+  TORCH_CHECK(fp4_dtype(dtype) >= 0, "ashqk: dequantize_fp4 supports float16, bfloat16 and float32");
+  check_fp4(codes, scales, K, format, codes.device());
+  c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor out = at::empty({codes.size(0), K}, codes.options().dtype(dtype));
+  if (codes.size(0) == 0) return out;
+  check_rc(ashqk_dequantize_fp4(codes.data_ptr(), codes_ld(codes), scales.data_ptr(), out.data_ptr(), K, fp4_dtype(dtype),
+                                static_cast<int>(codes.size(0)), static_cast<int>(K), static_cast<int>(format),
+                                static_cast<float>(global_scale),
+                                c10::cuda::getCurrentCUDAStream(codes.device().index()).stream()),
+           "dequantize_fp4");
+  return out;
+}
+
+at::Tensor fp4_matmul(const at::Tensor& a_codes, const at::Tensor& a_scales, const at::Tensor& b_codes,
+                      const at::Tensor& b_scales, int64_t K, int64_t format, double alpha, at::ScalarType dtype) {
+  TORCH_CHECK(a_codes.is_cuda(), "ashqk: codes must be CUDA tensors");
+  TORCH_CHECK(dtype == at::kHalf || dtype == at::kBFloat16, "ashqk: fp4_matmul returns float16 or bfloat16");
+  check_fp4(a_codes, a_scales, K, format, a_codes.device());
+  check_fp4(b_codes, b_scales, K, format, a_codes.device());
+  c10::cuda::CUDAGuard guard(a_codes.device());
+  const int64_t M = a_codes.size(0), N = b_codes.size(0);
+  at::Tensor y = at::empty({M, N}, a_codes.options().dtype(dtype));
+  if (M == 0 || N == 0) return y;
+  check_rc(ashqk_fp4_matmul(a_codes.data_ptr(), codes_ld(a_codes), a_scales.data_ptr(), b_codes.data_ptr(),
+                            codes_ld(b_codes), b_scales.data_ptr(), y.data_ptr(), N, fp4_dtype(dtype), static_cast<int>(M),
+                            static_cast<int>(N), static_cast<int>(K), static_cast<int>(format), static_cast<float>(alpha),
+                            c10::cuda::getCurrentCUDAStream(a_codes.device().index()).stream()),
+           "fp4_matmul");
+  return y;
+}
+
+at::Tensor w4a4_linear(const at::Tensor& x, const at::Tensor& codes, const at::Tensor& scales, int64_t K,
+                       int64_t format, double x_scale, double w_scale, bool gated) {
+  TORCH_CHECK(x.is_cuda(), "ashqk: x must be a CUDA tensor");
+  const int dtype = fp4_dtype(x.scalar_type());
+  TORCH_CHECK((dtype == ASHQK_F16 || dtype == ASHQK_BF16) && x.dim() >= 1, "ashqk: x must be a float16 or bfloat16 tensor");
+  check_no_grad(x, "w4a4_linear");
+  const int64_t cols = gated ? 2 * K : K;
+  TORCH_CHECK(x.size(-1) == cols, "ashqk: x must have ", cols, " columns for weights of K = ", K, gated ? " (gated)" : "");
+  check_fp4(codes, scales, K, format, x.device());
+  c10::cuda::CUDAGuard guard(x.device());
+  const Rows r = as_rows(x, cols);
+  const int64_t N = codes.size(0);
+  at::Tensor y = at::empty({r.rows, N}, x.options());
+  if (r.rows > 0 && N > 0) {
+    size_t bytes = 0;
+    check_rc(ashqk_w4a4_workspace_size(static_cast<int>(r.rows), static_cast<int>(N), static_cast<int>(K), static_cast<int>(format), &bytes), "w4a4_linear");
+    // Holds x quantised between two launches; from PyTorch's allocator, so streams and graphs each have their own.
+    at::Tensor ws;
+    if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte));
+    check_rc(ashqk_w4a4_linear(r.t.data_ptr(), r.ld, dtype, gated, static_cast<float>(x_scale), codes.data_ptr(), codes_ld(codes),
+                               scales.data_ptr(), static_cast<float>(w_scale), y.data_ptr(), N, static_cast<int>(r.rows),
+                               static_cast<int>(N), static_cast<int>(K), static_cast<int>(format),
+                               bytes ? ws.data_ptr() : nullptr, bytes,
+                               c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+             "w4a4_linear");
+  }
+  if (x.dim() == 2) return y;
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  return y.view(shape);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(ashqk, m) {
@@ -183,6 +320,14 @@ TORCH_LIBRARY(ashqk, m) {
   m.def("w4a16_linear(Tensor x, Tensor qweight, Tensor qzeros, Tensor scales) -> Tensor");
   m.def("w4a16_linear_out(Tensor x, Tensor qweight, Tensor qzeros, Tensor scales, Tensor(a!) out) -> Tensor(a!)");
   m.def("dequantize_awq(Tensor qweight, Tensor qzeros, Tensor scales, ScalarType dtype) -> Tensor");
+  m.def("quantize_fp4(Tensor x, int format, float global_scale, bool gated) -> (Tensor, Tensor)");
+  m.def("dequantize_fp4(Tensor codes, Tensor scales, int K, int format, float global_scale, ScalarType dtype) -> Tensor");
+  m.def(
+      "fp4_matmul(Tensor a_codes, Tensor a_scales, Tensor b_codes, Tensor b_scales, int K, int format, float alpha, "
+      "ScalarType dtype) -> Tensor");
+  m.def(
+      "w4a4_linear(Tensor x, Tensor codes, Tensor scales, int K, int format, float x_scale, float w_scale, bool gated) "
+      "-> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(ashqk, CUDA, m) {
@@ -191,4 +336,8 @@ TORCH_LIBRARY_IMPL(ashqk, CUDA, m) {
   m.impl("w4a16_linear", &w4a16_linear);
   m.impl("w4a16_linear_out", &w4a16_linear_out);
   m.impl("dequantize_awq", &dequantize_awq);
+  m.impl("quantize_fp4", &quantize_fp4);
+  m.impl("dequantize_fp4", &dequantize_fp4);
+  m.impl("fp4_matmul", &fp4_matmul);
+  m.impl("w4a4_linear", &w4a4_linear);
 }

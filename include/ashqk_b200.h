@@ -316,6 +316,61 @@ ASHQK_API int ashqk_w4a16_gemv_allreduce(const void* x, int64_t x_ld, const int3
                                          const void* regions_dev, int rank, int world, int64_t max_elems,
                                          void* stream);
 
+/*
+ * Microscaled 4-bit floating point (MXFP4 / NVFP4), beside the AWQ integers. No reference counterpart:
+ * the reference holds weights in 4 bits and multiplies in 16; here both operands of a product are
+ * 4-bit and go to the tensor core as they are.
+ *
+ * An element is E2M1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and negatives); a block of a row's columns shares one
+ * scale. ASHQK_MXFP4: 32 columns, scale 2^(floor(log2 amax) - 2) as E8M0. ASHQK_NVFP4: 16 columns,
+ * scale E4M3(min(448, amax / (6 g))) times a global scale g of the tensor (1e-18 .. 1e18). An element
+ * is its value over the scale, to nearest even, held to +-6. A block holding an infinity or a NaN
+ * gets the NaN scale and reads back as NaN.
+ *
+ *   codes   uint8 [M, Kp/2]  Kp = K rounded up to 32; two to a byte, the even column low; the padding
+ *                            columns are zero; row stride codes_ld bytes, a multiple of 16
+ *   scales  uint8            [ceil(M/128)][ceil(blocks/4)][row % 32][row / 32 % 4][block % 4] with blocks
+ *                            = Kp / block size; contiguous; padding blocks hold 0, padding rows anything
+ *
+ * ashqk_fp4_sizes gives the smallest codes_ld and the bytes of scales. codes and scales are 16-byte
+ * aligned. For ASHQK_MXFP4 the global scale has to be 1.
+ */
+typedef enum ashqk_fp4_format { ASHQK_MXFP4 = 0, ASHQK_NVFP4 = 1 } ashqk_fp4_format;
+typedef enum ashqk_dtype { ASHQK_F16 = 0, ASHQK_BF16 = 1, ASHQK_F32 = 2 } ashqk_dtype;
+
+ASHQK_API int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int64_t* scales_bytes);
+
+/*
+ * x [M, K] (ashqk_dtype, row stride x_ld elements) -> codes, scales. With gated != 0, x is [M, 2 K] and
+ * what is quantised is silu(x[:, :K]) * x[:, K:], computed in fp32 and rounded once, to the format.
+ */
+ASHQK_API int ashqk_quantize_fp4(const void* x, int64_t x_ld, int dtype, int gated, void* codes, int64_t codes_ld,
+                                 void* scales, int M, int K, int format, float global_scale, void* stream);
+
+/* codes, scales -> out [M, K] (ashqk_dtype, row stride out_ld elements). */
+ASHQK_API int ashqk_dequantize_fp4(const void* codes, int64_t codes_ld, const void* scales, void* out, int64_t out_ld,
+                                   int dtype, int M, int K, int format, float global_scale, void* stream);
+
+/*
+ * y [M, N] (ashqk_dtype F16 or BF16, row stride y_ld elements) = alpha * A @ B^T for quantised A [M, K] and
+ * B [N, K] of one format; alpha carries the global scales' product. fp32 accumulation.
+ */
+ASHQK_API int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes,
+                               int64_t b_ld, const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K,
+                               int format, float alpha, void* stream);
+
+/*
+ * W4A4 linear layer: y [M, N] = Q(x) @ W^T with 16-bit x [M, K] quantised on the way (to the weights' format,
+ * with global scale x_scale) and W [N, K] held quantised (global scale w_scale). dtype is x's and y's (F16
+ * or BF16); gated as in ashqk_quantize_fp4 (x is [M, 2 K]). Few rows are quantised inside the product's
+ * one launch; for more, the workspace of ashqk_w4a4_workspace_size bytes (16-byte aligned, contents
+ * irrelevant, written) holds Q(x) between two launches.
+ */
+ASHQK_API int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes);
+ASHQK_API int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gated, float x_scale, const void* w_codes,
+                                int64_t w_ld, const void* w_scales, float w_scale, void* y, int64_t y_ld, int M, int N,
+                                int K, int format, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
