@@ -300,8 +300,6 @@ int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, cudaStream_
 
 }  // namespace
 
-int check_fp4_operand(const void* codes, int64_t codes_ld, const void* scales, int K);
-
 int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
                     const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
                     cudaStream_t stream) {
@@ -332,16 +330,3 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
 }
 
 }  // namespace ashqk
-
-using namespace ashqk;
-
-extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
-                                const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format,
-                                float alpha, void* stream) {
-  if (!y || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || y_ld < N || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
-  if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
-  if (const int rc = check_fp4_operand(a_codes, a_ld, a_scales, K)) return rc;
-  if (const int rc = check_fp4_operand(b_codes, b_ld, b_scales, K)) return rc;
-  return fp4_matmul_rows(a_codes, a_ld, a_scales, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N, K, format, alpha,
-                         static_cast<cudaStream_t>(stream));
-}

@@ -1,4 +1,6 @@
 // W4A4 linear layer: x in 16 bits, quantised on the way into the product with 4-bit weights.
+#include <atomic>
+
 #include "fp4.cuh"
 
 namespace ashqk {
@@ -9,7 +11,16 @@ bool fp4_global_scale_ok(int format, float gs);
 int quantize_fp4(const void* x, int64_t x_ld, int dtype, bool gated, void* codes, int64_t codes_ld, void* scales, int M,
                  int K, int format, float gs, bool early, cudaStream_t stream);
 
+int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
+                    const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
+                    cudaStream_t stream);
+int fp4_matmul_pair(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
+                    const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
+                    cudaStream_t stream);
+
 namespace {
+
+std::atomic<int> g_matmul_kernel{0};
 
 // Q(x) in the workspace: scales first (a multiple of 512 bytes), then codes.
 void workspace_layout(int M, int K, int format, size_t* codes_offset, size_t* bytes) {
@@ -21,6 +32,25 @@ void workspace_layout(int M, int K, int format, size_t* codes_offset, size_t* by
 }  // namespace ashqk
 
 using namespace ashqk;
+
+extern "C" int ashqk_set_fp4_kernel(int which) {
+  if (which < 0 || which > 2) return ASHQK_ERR_INVALID_ARGUMENT;
+  g_matmul_kernel.store(which, std::memory_order_relaxed);
+  return ASHQK_OK;
+}
+
+extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
+                                const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format,
+                                float alpha, void* stream) {
+  if (!y || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || y_ld < N || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (const int rc = check_fp4_operand(a_codes, a_ld, a_scales, K)) return rc;
+  if (const int rc = check_fp4_operand(b_codes, b_ld, b_scales, K)) return rc;
+  const int which = g_matmul_kernel.load(std::memory_order_relaxed);
+  const bool pair = which ? which == 2 : M > 128;
+  return (pair ? fp4_matmul_pair : fp4_matmul_rows)(a_codes, a_ld, a_scales, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N,
+                                                    K, format, alpha, static_cast<cudaStream_t>(stream));
+}
 
 extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes) {
   if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;

@@ -371,6 +371,12 @@ ASHQK_API int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gate
                                 int64_t w_ld, const void* w_scales, float w_scale, void* y, int64_t y_ld, int M, int N,
                                 int K, int format, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Tuning and test switch (process-wide): which product kernel the two calls above use. 0 automatic,
+ * 1 rows (128 rows of B by up to 256 of A per CTA, K split over a cluster), 2 CTA pairs (256 x 256).
+ */
+ASHQK_API int ashqk_set_fp4_kernel(int which);
+
 #ifdef __cplusplus
 }
 #endif

@@ -176,6 +176,36 @@ def test_matmul(fmt, m, n, k):
     check_product(ashqk.fp4_matmul(a, b, dtype), a64, b64)
 
 
+@pytest.fixture(params=[1, 2], ids=["rows", "pair"])
+def forced(request):
+    """Each product kernel for sizes that the rule gives to the other."""
+    import ctypes
+
+    from ashqk import _ext
+
+    lib = ctypes.CDLL(_ext.C_LIBRARY)
+    assert lib.ashqk_set_fp4_kernel(request.param) == 0
+    yield request.param
+    assert lib.ashqk_set_fp4_kernel(0) == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (3, 300, 96), (128, 128, 64), (129, 513, 288), (256, 256, 256), (600, 520, 1312), (1500, 2900, 512)])
+def test_matmul_either_kernel(forced, fmt, m, n, k):
+    a, a64 = random_operand(m, k, fmt, m)
+    b, b64 = random_operand(n, k, fmt, n * 3)
+    check_product(ashqk.fp4_matmul(a, b), a64, b64)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_matmul_many_tiles_per_pair(fmt):
+    """More tiles than the persistent kernel's pairs hold at once, an odd number of them each."""
+    m, n, k = 256 * 11 + 5, 256 * 23 + 9, 320
+    a, a64 = random_operand(m, k, fmt, 1)
+    b, b64 = random_operand(n, k, fmt, 2)
+    check_product(ashqk.fp4_matmul(a, b), a64, b64)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_matmul_each_code_and_scale_place(fmt):
     """One nonzero column at a time: every code, block and row of a scale tile lands where it belongs."""
