@@ -6,8 +6,8 @@
 // weights' bytes: a CTA owns 128 weight rows and a slice of K, the CTAs of a cluster split K and add
 // their partial sums over distributed shared memory in rank order, so a result does not depend on timing.
 //
-//   warp 0      one thread: TMA of codes, bulk copies of scale tiles, kRing stages
-//   warp 1      one thread: tcgen05.cp of a stage's scales, its four MMAs, commit
+//   warp 0      one elected lane: TMA of codes, bulk copies of scale tiles
+//   warp 1      one elected lane: tcgen05.cp of a stage's scales, its four MMAs, commit
 //   warps 2..5  after the last MMA: TMEM -> registers -> y, or -> shared memory and the cluster's sum
 //
 // The scales' TMEM columns are double-buffered: stage i's copies wait for the MMAs of stage i - 2. All
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known to be uniform
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % a.cluster;
   const int tile = static_cast<int>(blockIdx.x) / a.cluster;
@@ -117,67 +117,86 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
   pdl_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
-      const int x_tiles = min(L::kXTiles, (a.M - m0 + 127) / 128);
-      int stage = 0;
-      uint32_t phase = 0;
-      int issued = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, abort, true)) break;
-        unsigned char* base = smem + stage * L::kStage;
-        const int t0 = kb * L::kT;
-        const uint32_t sf = static_cast<uint32_t>(min(L::kT, a.scale_tiles - t0)) * kFp4TileBytes;
+    const int x_tiles = min(L::kXTiles, (a.M - m0 + 127) / 128);
+    int stage = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(&empty[stage], phase ^ 1u, abort, true)) break;
+      unsigned char* base = smem + stage * L::kStage;
+      const int t0 = kb * L::kT;
+      const uint32_t sf = static_cast<uint32_t>(min(L::kT, a.scale_tiles - t0)) * kFp4TileBytes;
+      if (elect_one()) {
         mbar_arrive_expect_tx(&full[stage], L::kW + L::kX + sf * (1 + x_tiles));
         tma_load_2d(base, &maps.w, kb * 128, n0, &full[stage]);
-        tma_load_2d(base + L::kW, &maps.x, kb * 128, m0, &full[stage]);
         bulk_load(base + L::kW + L::kX, a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+        tma_load_2d(base + L::kW, &maps.x, kb * 128, m0, &full[stage]);
         for (int t = 0; t < x_tiles; ++t)
           bulk_load(base + L::kW + L::kX + L::kWS + t * L::kWS,
                     a.xs + (static_cast<int64_t>(m0 / 128 + t) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
-        ++issued;
-        if (++stage == a.ring) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
-      for (int i = 1; i <= a.ring && i <= issued; ++i) {
-        const int f = issued - i;
-        mbar_drain(&full[f % a.ring], static_cast<uint32_t>(f / a.ring) & 1u);
+      __syncwarp();
+      ++issued;
+      if (++stage == a.ring) {
+        stage = 0;
+        phase ^= 1u;
       }
     }
+    for (int i = 1; i <= a.ring && i <= issued; ++i) {
+      const int f = issued - i;
+      mbar_drain(&full[f % a.ring], static_cast<uint32_t>(f / a.ring) & 1u);
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        const int i = kb - kb0;
-        const int stage = i % a.ring;
-        if (!mbar_wait(&full[stage], static_cast<uint32_t>(i / a.ring) & 1u, abort, true)) break;
-        if (i >= 2 && !mbar_wait(&empty[(i - 2) % a.ring], static_cast<uint32_t>((i - 2) / a.ring) & 1u, abort, true)) break;
-        tc_fence_after_sync();
-        const uint32_t base = sbase + stage * L::kStage;
-        const uint32_t sfw = tmem + L::kSf0 + (i & 1) * (L::kSfW + L::kSfX);
-        const uint32_t sfx = sfw + L::kSfW;
-        const int steps = min(4, a.k_steps - kb * 4);
-        const int tiles = Mma::tile_of(steps - 1) + 1;
+    int stage = 0, old = 0;  // stage of kb, of kb - 2
+    uint32_t phase = 0, old_phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0;
+      if (!mbar_wait(&full[stage], phase, abort, true)) break;
+      if (i >= 2) {
+        if (!mbar_wait(&empty[old], old_phase, abort, true)) break;
+        if (++old == a.ring) {
+          old = 0;
+          old_phase ^= 1u;
+        }
+      }
+      tc_fence_after_sync();
+      const uint32_t base = sbase + stage * L::kStage;
+      const uint32_t sfw = tmem + L::kSf0 + (i & 1) * (L::kSfW + L::kSfX);
+      const uint32_t sfx = sfw + L::kSfW;
+      const uint64_t sd = scale_tile_desc(base + L::kW + L::kX);
+      const uint64_t dw = umma_desc_sw128(base, 16u, 1024u);
+      const uint64_t dx = umma_desc_sw128(base + L::kW, 16u, 1024u);
+      const int steps = min(4, a.k_steps - kb * 4);
+      const int tiles = Mma::tile_of(steps - 1) + 1;
+      if (elect_one()) {
 #pragma unroll
         for (int t = 0; t < L::kT; ++t) {
           if (t >= tiles) break;
-          scale_tile_to_tmem(sfw + t * 4, scale_tile_desc(base + L::kW + L::kX + t * kFp4TileBytes));
+          scale_tile_to_tmem(sfw + t * 4, sd + t * (kFp4TileBytes >> 4));
+#pragma unroll
           for (int r = 0; r < L::kXTiles; ++r)
-            scale_tile_to_tmem(sfx + (t * L::kXTiles + r) * 4,
-                               scale_tile_desc(base + L::kW + L::kX + L::kWS + r * L::kWS + t * kFp4TileBytes));
+            scale_tile_to_tmem(sfx + (t * L::kXTiles + r) * 4, sd + (((1 + r) * L::kWS + t * kFp4TileBytes) >> 4));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j >= steps) break;
-          Mma::mma(tmem, umma_desc_sw128(base + 32u * j, 16u, 1024u), umma_desc_sw128(base + L::kW + 32u * j, 16u, 1024u),
-                   Mma::idesc(kTileN, NT, j), sfw + Mma::tile_of(j) * 4, sfx + Mma::tile_of(j) * L::kXTiles * 4,
-                   (i | j) != 0);
+          Mma::mma(tmem, dw + 2 * j, dx + 2 * j, Mma::idesc(kTileN, NT, j), sfw + Mma::tile_of(j) * 4,
+                   sfx + Mma::tile_of(j) * L::kXTiles * 4, (i | j) != 0);
         }
         umma_commit(&empty[stage]);
+        if (kb + 1 == kb1) umma_commit(done);
       }
-      umma_commit(done);
-      mbar_drain(done, 0);
+      __syncwarp();
+      if (++stage == a.ring) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    if (*abort) {  // the commit above may not have been reached
+      if (elect_one()) umma_commit(done);
+      __syncwarp();
+    }
+    mbar_drain(done, 0);
   } else {
     const int quad = warp & 3;
     const bool ok = mbar_wait(done, 0, abort);
