@@ -162,19 +162,30 @@ __device__ __forceinline__ void unpack2<__nv_bfloat16>(uint32_t u, float& lo, fl
   hi = __uint_as_float(u & 0xffff0000u);
 }
 
+// Read once, and not through the read-only path: with programmatic dependent launch the previous kernel may still be
+// writing when this one starts.
+__device__ __forceinline__ uint4 ld_once_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+
 // Eight consecutive values: `vec` when p is 16-byte aligned and all eight exist, else one by one with
 // zeros from `count` on.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
   if (vec) {
     if (sizeof(T) == 2) {
-      const uint4 u = ld_stream_v4(p);
+      const uint4 u = ld_once_v4(p);
       unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.x, v[0], v[1]);
       unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.y, v[2], v[3]);
       unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.z, v[4], v[5]);
       unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.w, v[6], v[7]);
     } else {
-      const uint4 a = ld_stream_v4(p), b = ld_stream_v4(p + 4);
+      const uint4 a = ld_once_v4(p), b = ld_once_v4(p + 4);
       v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
       v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
     }

@@ -1,14 +1,20 @@
-// y = alpha * A B^T with 4-bit operands, for any number of rows of A; made for few.
+// y = alpha * A B^T with 4-bit operands, for any number of rows of A; made for few. A comes quantised, or
+// (up to 16 rows) in 16 bits and is quantised here.
 //
 // The weights' rows (B, N of them) take the tensor core's 128-row side and A's rows its column side, so that
 // one token wastes 7 of 8 columns instead of 127 of 128 rows, and every weight byte goes from HBM
 // through shared memory to the tensor core with no instruction touching it. With few rows the floor is the
 // weights' bytes: a CTA owns 128 weight rows and a slice of K, the CTAs of a cluster split K and add
-// their partial sums over distributed shared memory in rank order, so a result does not depend on timing.
+// their partial sums in rank order, so a result does not depend on timing.
 //
-//   warp 0      one elected lane: TMA of codes, bulk copies of scale tiles
+//   warp 0      one elected lane: prefetches its weights into L2 before the previous kernel has ended
+//               (L2 is coherent, so what that kernel may still write is not missed), then TMA of codes and
+//               bulk copies of scale tiles
 //   warp 1      one elected lane: tcgen05.cp of a stage's scales, its four MMAs, commit
-//   warps 2..5  after the last MMA: TMEM -> registers -> y, or -> shared memory and the cluster's sum
+//   warps 2..9  fused form: quantise this CTA's slice of A into shared memory, in the layout in which TMA and
+//               the scale tiles arrive otherwise; then warps 2..5: TMEM -> registers -> y, or, with a split K,
+//               -> the shared memory of the CTA that adds these rows of A (st.async, counted in bytes on
+//               its barrier)
 //
 // The scales' TMEM columns are double-buffered: stage i's copies wait for the MMAs of stage i - 2. All
 // waits are bounded.
@@ -21,7 +27,10 @@ namespace ashqk {
 namespace {
 
 constexpr int kTileN = 128;  // weight rows per CTA
-constexpr int kThreads = 192;
+constexpr int kQuantWarps = 8;
+constexpr int kThreads = 64 + 32 * kQuantWarps;
+constexpr int kMaxRing = 12;
+constexpr int kMaxCluster = 8;
 
 struct RowsMaps {
   CUtensorMap w, x;
@@ -29,69 +38,132 @@ struct RowsMaps {
 
 struct RowsArgs {
   const uint8_t* ws;  // scales
-  const uint8_t* xs;
+  const uint8_t* xs;  // scales of a quantised A
+  const void* x;      // A in 16 bits (fused)
+  int64_t x_ld;
   void* y;
   int64_t y_ld;
-  int M, N, k_steps, num_kb, scale_tiles;  // k_steps: MMAs of 64 columns over all of K
+  int M, N, K, k_steps, num_kb, scale_tiles;  // k_steps: MMAs of 64 columns over all of K
   int cluster, ring;
-  float alpha;
-  int bf16;
+  uint32_t off_x, off_slots, off_bar;  // shared memory after the ring
+  float alpha, x_gs;
+  int bf16, gated, vec;
 };
 
-template <int FMT, int NT>
-struct RowsSmem {
+template <int FMT, int NT, bool FUSED>
+struct RowsShape {
   static constexpr int kT = Fp4Mma<FMT>::kTilesPerStage;
   static constexpr int kXTiles = NT > 128 ? 2 : 1;  // 128-row scale tiles of A's rows
   static constexpr uint32_t kW = kTileN * 128;
-  static constexpr uint32_t kX = NT * 128;
   static constexpr uint32_t kWS = kT * kFp4TileBytes;
+  static constexpr uint32_t kX = NT * 128;
   static constexpr uint32_t kXS = kXTiles * kT * kFp4TileBytes;
-  static constexpr uint32_t kStage = kW + kX + kWS + kXS;
-  static constexpr uint32_t kPartial = NT * kTileN * 4;
+  static constexpr uint32_t kStage = kW + kWS + (FUSED ? 0 : kX + kXS);
   static_assert(kStage % 1024 == 0, "swizzle atoms need 1 KB alignment");
-  static constexpr int kMaxRing = 12;
-  static constexpr uint32_t kMisc = (2 * kMaxRing + 2) * 8 + 16;
+  // Fused: the quantised slice, [stage][row][128] and after it the scale tiles, of which only the first NT rows
+  // are there: the copy to TMEM reads on into the next tile, for rows that nobody uses.
+  static constexpr uint32_t kXSTile = NT * 16;
   // TMEM: the sums, then two buffers of scales.
   static constexpr int kSfW = kT * 4, kSfX = kXTiles * kT * 4;
   static constexpr int kSf0 = NT < 32 ? 32 : NT;
   static constexpr int kCols = kSf0 + 2 * (kSfW + kSfX);
   static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
   static_assert(kCols <= 512, "TMEM");
+  // Split K: whether the slots for partial sums have shared memory of their own or take the ring's.
+  static constexpr bool kOwnSlots = NT <= 32;
+  static constexpr uint32_t slots(int cluster) {
+    return static_cast<uint32_t>(((NT / 4 + cluster - 1) / cluster) * cluster) * kTileN * 16;
+  }
 };
 
-template <typename T>
-__device__ __forceinline__ void store4(T* y, const float (&v)[4], int count, bool vec) {
-  if (vec && count >= 4) {
-    *reinterpret_cast<uint2*>(y) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-  } else {
+__device__ __forceinline__ void st_async_v4(uint32_t remote_addr, uint4 v, uint32_t remote_bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
+                   remote_addr),
+               "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(remote_bar)
+               : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+__device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
+}
+
+// Quantises columns [256 kb0, 256 kb1) of A's rows into shared memory. Eight columns per thread, a block's
+// lanes adjacent, as in the quantiser proper.
+template <int FMT, int NT, typename T>
+__device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int kb1, uint32_t codes, uint32_t scales, int tid) {
+  using L = RowsShape<FMT, NT, true>;
+  constexpr int kLanes = fp4_block(FMT) / 8;
+  const int chunks = (kb1 - kb0) * 32;
+  const int total = a.M * chunks;  // a multiple of 32: warps stay whole
+  const T* x = static_cast<const T*>(a.x);
+  for (int i = tid; i < total; i += 32 * kQuantWarps) {
+    const int m = i / chunks;
+    const int c = i - m * chunks;
+    const int k0 = kb0 * kFp4BlockK + c * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k0 < a.K) {
+      const T* p = x + m * a.x_ld + k0;
+      const bool whole = a.vec && k0 + 8 <= a.K;
+      load8<T>(p, a.K - k0, whole, v);
+      if (a.gated) {
+        float u[8];
+        load8<T>(p + a.K, a.K - k0, whole, u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < count) y[i] = from_f32<T>(v[i]);
+        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
+      }
+    }
+    uint32_t amax = abs_max8(v);
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    float divisor;
+    const uint32_t byte = fp4_scale_of<FMT>(amax, a.x_gs, &divisor);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], divisor);
+    const int kb = c >> 5, cc = c & 31;
+    const uint32_t at = codes + kb * L::kX + (m >> 3) * 1024 + (m & 7) * 128 + (((cc >> 2) ^ (m & 7)) << 4) + (cc & 3) * 4;
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(fp4_pack8(v)) : "memory");
+    if (cc % kLanes == 0) {
+      const int block = cc / kLanes;
+      const uint32_t s = scales + (kb * L::kT + (block >> 2)) * L::kXSTile + m * 16 + (block & 3);
+      asm volatile("st.shared.u8 [%0], %1;" ::"r"(s), "r"(byte) : "memory");
+    }
   }
 }
 
-template <int FMT, int NT>
+template <int FMT, int NT, bool FUSED>
 __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs a) {
-  using L = RowsSmem<FMT, NT>;
+  using L = RowsShape<FMT, NT, FUSED>;
   using Mma = Fp4Mma<FMT>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = smem_u32(smem);
-  const uint32_t data = max(static_cast<uint32_t>(a.ring) * L::kStage, a.cluster > 1 ? L::kPartial : 0u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + data);
-  uint64_t* empty = full + L::kMaxRing;
-  uint64_t* done = empty + L::kMaxRing;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + a.off_bar);
+  uint64_t* empty = full + kMaxRing;
+  uint64_t* done = empty + kMaxRing;
+  uint64_t* x_ready = done + 1;
+  uint64_t* received = x_ready + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(received + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);  // known to be uniform
   const int lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(blockIdx.x) % a.cluster;
-  const int tile = static_cast<int>(blockIdx.x) / a.cluster;
+  const int C = a.cluster;
+  const int rank = static_cast<int>(blockIdx.x) % C;
+  const int tile = static_cast<int>(blockIdx.x) / C;
   const int n0 = tile * kTileN;
   const int m0 = static_cast<int>(blockIdx.y) * NT;
-  const int kb0 = static_cast<int>(static_cast<int64_t>(a.num_kb) * rank / a.cluster);
-  const int kb1 = static_cast<int>(static_cast<int64_t>(a.num_kb) * (rank + 1) / a.cluster);
+  const int kb0 = static_cast<int>(static_cast<int64_t>(a.num_kb) * rank / C);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(a.num_kb) * (rank + 1) / C);
+  // Groups of four rows of A; group g's partial sums are added by the CTA of rank g % C.
+  const int groups = (min(NT, a.M - m0) + 3) / 4;
+  const int my_groups = (groups - rank + C - 1) / C;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.ring; ++s) {
@@ -99,10 +171,22 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
+    mbar_init(x_ready, kQuantWarps);
+    mbar_init(received, 1);
     *abort = 0;
     fence_mbarrier_init();
+    if (C > 1) mbar_arrive_expect_tx(received, static_cast<uint32_t>(my_groups * C) * kTileN * 16);
+  }
+  __syncthreads();
+  // This CTA's barriers can be signalled (waited for before the first remote store). Before the allocation, which
+  // can wait for CTAs of other clusters on this SM.
+  if (C > 1) cluster_arrive();
+  if (warp == 0 && elect_one()) {
     prefetch_tensormap(&maps.w);
-    prefetch_tensormap(&maps.x);
+    for (int kb = kb0; kb < kb1; ++kb) l2_prefetch_2d(&maps.w, kb * 128, n0);
+    const int t0 = kb0 * L::kT, t1 = min(kb1 * L::kT, a.scale_tiles);
+    l2_prefetch(a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, (t1 - t0) * kFp4TileBytes);
+    if (!FUSED) prefetch_tensormap(&maps.x);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, L::kTmemCols);
@@ -111,13 +195,17 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-
-  pdl_wait();
+  // After the allocation: a CTA of the next launch that holds TMEM on this SM waits for this grid, which must
+  // not still be waiting for TMEM.
   pdl_launch_dependents();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  pdl_wait();
+
+  const uint32_t x_codes = sbase + a.off_x;
+  const uint32_t x_scales = x_codes + static_cast<uint32_t>(kb1 - kb0) * L::kX;
 
   if (warp == 0) {
-    const int x_tiles = min(L::kXTiles, (a.M - m0 + 127) / 128);
+    const int x_tiles = FUSED ? 0 : min(L::kXTiles, (a.M - m0 + 127) / 128);
     int stage = 0;
     uint32_t phase = 0;
     int issued = 0;
@@ -127,13 +215,15 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
       const int t0 = kb * L::kT;
       const uint32_t sf = static_cast<uint32_t>(min(L::kT, a.scale_tiles - t0)) * kFp4TileBytes;
       if (elect_one()) {
-        mbar_arrive_expect_tx(&full[stage], L::kW + L::kX + sf * (1 + x_tiles));
+        mbar_arrive_expect_tx(&full[stage], L::kW + (FUSED ? 0 : L::kX) + sf * (1 + x_tiles));
         tma_load_2d(base, &maps.w, kb * 128, n0, &full[stage]);
-        bulk_load(base + L::kW + L::kX, a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
-        tma_load_2d(base + L::kW, &maps.x, kb * 128, m0, &full[stage]);
-        for (int t = 0; t < x_tiles; ++t)
-          bulk_load(base + L::kW + L::kX + L::kWS + t * L::kWS,
-                    a.xs + (static_cast<int64_t>(m0 / 128 + t) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+        bulk_load(base + L::kW, a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+        if (!FUSED) {
+          tma_load_2d(base + L::kW + L::kWS, &maps.x, kb * 128, m0, &full[stage]);
+          for (int t = 0; t < x_tiles; ++t)
+            bulk_load(base + L::kW + L::kWS + L::kX + t * L::kWS,
+                      a.xs + (static_cast<int64_t>(m0 / 128 + t) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+        }
       }
       __syncwarp();
       ++issued;
@@ -149,11 +239,18 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
   } else if (warp == 1) {
     int stage = 0, old = 0;  // stage of kb, of kb - 2
     uint32_t phase = 0, old_phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    bool ok = !FUSED || mbar_wait(x_ready, 0, abort, true);
+    for (int kb = kb0; ok && kb < kb1; ++kb) {
       const int i = kb - kb0;
-      if (!mbar_wait(&full[stage], phase, abort, true)) break;
+      if (!mbar_wait(&full[stage], phase, abort, true)) {
+        ok = false;
+        break;
+      }
       if (i >= 2) {
-        if (!mbar_wait(&empty[old], old_phase, abort, true)) break;
+        if (!mbar_wait(&empty[old], old_phase, abort, true)) {
+          ok = false;
+          break;
+        }
         if (++old == a.ring) {
           old = 0;
           old_phase ^= 1u;
@@ -163,9 +260,10 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
       const uint32_t base = sbase + stage * L::kStage;
       const uint32_t sfw = tmem + L::kSf0 + (i & 1) * (L::kSfW + L::kSfX);
       const uint32_t sfx = sfw + L::kSfW;
-      const uint64_t sd = scale_tile_desc(base + L::kW + L::kX);
+      const uint64_t sd = scale_tile_desc(base + L::kW);
+      const uint64_t sx = scale_tile_desc(FUSED ? x_scales + i * L::kT * L::kXSTile : base + L::kW + L::kWS + L::kX);
       const uint64_t dw = umma_desc_sw128(base, 16u, 1024u);
-      const uint64_t dx = umma_desc_sw128(base + L::kW, 16u, 1024u);
+      const uint64_t dx = umma_desc_sw128(FUSED ? x_codes + i * L::kX : base + L::kW + L::kWS, 16u, 1024u);
       const int steps = min(4, a.k_steps - kb * 4);
       const int tiles = Mma::tile_of(steps - 1) + 1;
       if (elect_one()) {
@@ -173,9 +271,13 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
         for (int t = 0; t < L::kT; ++t) {
           if (t >= tiles) break;
           scale_tile_to_tmem(sfw + t * 4, sd + t * (kFp4TileBytes >> 4));
+          if (FUSED) {
+            scale_tile_to_tmem(sfx + t * 4, sx + t * (L::kXSTile >> 4));
+          } else {
 #pragma unroll
-          for (int r = 0; r < L::kXTiles; ++r)
-            scale_tile_to_tmem(sfx + (t * L::kXTiles + r) * 4, sd + (((1 + r) * L::kWS + t * kFp4TileBytes) >> 4));
+            for (int r = 0; r < L::kXTiles; ++r)
+              scale_tile_to_tmem(sfx + (t * L::kXTiles + r) * 4, sx + ((r * L::kWS + t * kFp4TileBytes) >> 4));
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -192,96 +294,159 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
         phase ^= 1u;
       }
     }
-    if (*abort) {  // the commit above may not have been reached
+    if (!ok) {  // the commit of the last stage was not reached
       if (elect_one()) umma_commit(done);
       __syncwarp();
     }
     mbar_drain(done, 0);
-  } else {
-    const int quad = warp & 3;
-    const bool ok = mbar_wait(done, 0, abort);
+  } else if (FUSED) {
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    if (a.bf16)
+      quantize_slice<FMT, NT, __nv_bfloat16>(a, kb0, kb1, x_codes, x_scales, tid);
+    else
+      quantize_slice<FMT, NT, __half>(a, kb0, kb1, x_codes, x_scales, tid);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(x_ready);
+  }
+
+  // ---- sums: warps 2..5, one lane per weight row ----
+  const bool epilogue = warp >= 2 && warp < 6;
+  const int row = 32 * (warp & 3) + lane;
+  const int n = n0 + row;
+  bool ok = false;
+  if (epilogue) {
+    ok = mbar_wait(done, 0, abort);
     tc_fence_after_sync();
-    const int row = 32 * quad + lane;  // weight row of the tile
-    const int n = n0 + row;
-    float* partial = reinterpret_cast<float*>(smem);
-    const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * quad) << 16);
-    if (ok) {
+  }
+  if (C > 1) {
+    __syncwarp();
+    cluster_wait();
+    if (!L::kOwnSlots) {  // every CTA of the cluster is through with its ring
+      __syncthreads();
+      cluster_sync();
+    }
+  }
+  const uint32_t slots = sbase + (L::kOwnSlots ? a.off_slots : 0u);
+  auto store = [&](int m, float v) {
+    if (m >= a.M || n >= a.N) return;
+    if (a.bf16)
+      static_cast<__nv_bfloat16*>(a.y)[m * a.y_ld + n] = __float2bfloat16_rn(v * a.alpha);
+    else
+      static_cast<__half*>(a.y)[m * a.y_ld + n] = __float2half_rn(v * a.alpha);
+  };
+  if (epilogue) {
+    const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 8) {
-        if (m0 + c >= a.M) break;
-        uint32_t r[8];
-        tmem_ld_32x32b_x8(taddr + c, r);
-        tmem_wait_ld();
+    for (int g = 0; g < groups; g += 2) {
+      uint32_t r[8];
+      tmem_ld_32x32b_x8(taddr + 4 * g, r);
+      tmem_wait_ld();
+      if (!ok) {  // a wait ran out: the sums are not there; peers still get the bytes that they count
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int m = m0 + c + i;
-          if (m >= a.M) break;
-          if (a.cluster > 1) {
-            partial[(c + i) * kTileN + row] = __uint_as_float(r[i]);
-          } else if (n < a.N) {
-            const float v = a.alpha * __uint_as_float(r[i]);
-            if (a.bf16)
-              static_cast<__nv_bfloat16*>(a.y)[m * a.y_ld + n] = __float2bfloat16_rn(v);
-            else
-              static_cast<__half*>(a.y)[m * a.y_ld + n] = __float2half_rn(v);
-          }
+        for (int i = 0; i < 8; ++i) r[i] = 0x7fffffffu;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (g + h >= groups) break;
+        if (C == 1) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) store(m0 + 4 * (g + h) + i, __uint_as_float(r[4 * h + i]));
+        } else {
+          const int owner = (g + h) % C;
+          const uint32_t at = slots + static_cast<uint32_t>((((g + h) / C) * C + rank) * kTileN + row) * 16;
+          uint32_t remote, bar;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(owner));
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(received)), "r"(owner));
+          st_async_v4(remote, make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]), bar);
         }
       }
     }
   }
   tc_fence_before_sync();
   __syncthreads();
-  // TMEM goes back before the CTA waits for its cluster: a CTA that holds it waits for nobody, so CTAs of
-  // several clusters that share SMs cannot block one another in the allocation.
   if (warp == 1) {
     __syncwarp();
     tc_fence_after_sync();
     tmem_dealloc(tmem, L::kTmemCols);
   }
-  if (a.cluster > 1) {
-    // Partial sums of every CTA are in its shared memory, whose ring is drained. Each rank adds and stores a
-    // share of the tile.
-    cluster_sync();
-    const bool vec = (a.y_ld & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0;
-    const int quads = min(NT, a.M - m0) * (kTileN / 4);
-    for (int q = rank * kThreads + static_cast<int>(threadIdx.x); q < quads; q += a.cluster * kThreads) {
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int r = 0; r < a.cluster; ++r) {
-        const float4 p = ld_shared_cluster_v4(map_shared_rank(smem + q * 16, r));
-        s[0] += p.x, s[1] += p.y, s[2] += p.z, s[3] += p.w;
-      }
+  if (C > 1) {
+    __syncwarp();
+    cluster_arrive();
+    if (epilogue && my_groups > 0 && mbar_wait_cluster(received, 0, abort)) {
+#pragma unroll 1
+      for (int l = 0; l < my_groups; ++l) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < C; ++c) {
+          const uint4 p = lds_v4(slots + static_cast<uint32_t>((l * C + c) * kTileN + row) * 16);
+          s[0] += __uint_as_float(p.x), s[1] += __uint_as_float(p.y), s[2] += __uint_as_float(p.z), s[3] += __uint_as_float(p.w);
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] *= a.alpha;
-      const int m = m0 + q / (kTileN / 4);
-      const int n = n0 + q % (kTileN / 4) * 4;
-      if (n < a.N) {
-        if (a.bf16)
-          store4(static_cast<__nv_bfloat16*>(a.y) + m * a.y_ld + n, s, a.N - n, vec);
-        else
-          store4(static_cast<__half*>(a.y) + m * a.y_ld + n, s, a.N - n, vec);
+        for (int i = 0; i < 4; ++i) store(m0 + 4 * (l * C + rank) + i, s[i]);
       }
     }
-    cluster_sync();  // no CTA leaves while another reads its partial sums
+    __syncwarp();
+    cluster_wait();  // no CTA leaves while another may still store into it
   }
 }
 
-template <int FMT, int NT>
+std::atomic<int> g_cluster{0}, g_ring{0};
+
+// At least two stages: the wait for stage i - 2 counts on the producer not having passed it twice.
+struct RowsPlan {
+  int cluster, ring;
+  uint32_t off_x, off_slots, off_bar, smem;
+};
+
+// CTAs per cluster and stages in flight for `tiles` tiles of 128 weight rows (times the row blocks of A).
+template <int FMT, int NT, bool FUSED>
+RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
+  using L = RowsShape<FMT, NT, FUSED>;
+  RowsPlan p;
+  const int per_sm = L::kTmemCols <= 256 ? 2 : 1;
+  p.cluster = std::max(1, std::min({kMaxCluster, num_kb, sm_count * per_sm / std::max(1, tiles)}));
+  auto x_area = [&] {  // this CTA's slice of A, quantised
+    return FUSED ? ceil_div(num_kb, p.cluster) * (L::kX + L::kT * L::kXSTile) + kFp4TileBytes : 0u;
+  };
+  while (p.cluster < std::min(kMaxCluster, num_kb) && x_area() > 64 * 1024) ++p.cluster;
+  if (const int c = g_cluster.load(std::memory_order_relaxed)) p.cluster = std::min(c, num_kb);
+  const int local = ceil_div(num_kb, p.cluster);
+  const uint32_t x_bytes = x_area();
+  const uint32_t slots = p.cluster > 1 ? L::slots(p.cluster) : 0;
+  const uint32_t budget = per_sm == 2 ? 108 * 1024 : 218 * 1024;
+  const uint32_t fixed = x_bytes + (L::kOwnSlots ? slots : 0);
+  p.ring = fixed + 2 * L::kStage > budget ? 2 : static_cast<int>((budget - fixed) / L::kStage);
+  p.ring = std::max(2, std::min({kMaxRing, local, p.ring}));
+  if (const int r = g_ring.load(std::memory_order_relaxed)) p.ring = std::max(2, std::min({r, local, static_cast<int>((222 * 1024 - std::min(fixed, 222u * 1024)) / L::kStage)}));
+  uint32_t ring = p.ring * L::kStage;
+  if (!L::kOwnSlots) ring = std::max(ring, (slots + 1023) / 1024 * 1024);
+  p.off_x = ring;
+  p.off_slots = (p.off_x + x_bytes + 15) / 16 * 16;
+  p.off_bar = (p.off_slots + (L::kOwnSlots ? slots : 0) + 7) / 8 * 8;
+  p.smem = p.off_bar + (2 * kMaxRing + 3) * 8 + 16 + 1024;
+  // Without slots of their own, the CTAs of a cluster wait for one another while they hold TMEM. Two such CTAs on
+  // one SM must therefore both fit its 512 columns, or clusters could wait for each other's allocation in a
+  // circle: 128 columns always do (registers hold an SM to three CTAs), 256 are one to an SM, 512 alone.
+  if (!L::kOwnSlots && p.cluster > 1)
+    p.smem = std::max(p.smem, L::kTmemCols <= 128 ? 0u : L::kTmemCols == 256 ? 116u * 1024 : 200u * 1024);
+  return p;
+}
+
+template <int FMT, int NT, bool FUSED>
 int launch_rows(const RowsMaps& maps, RowsArgs a, cudaStream_t stream) {
-  using L = RowsSmem<FMT, NT>;
   DeviceInfo dev;
   if (const int rc = device_info(&dev)) return rc;
   const int tiles = ceil_div(a.N, kTileN);
   const int cols = ceil_div(a.M, NT);
   if (cols > 65535) return ASHQK_ERR_UNSUPPORTED;
-  // CTAs resident per SM by TMEM (512 columns), at most 2.
-  const int per_sm = L::kTmemCols <= 256 ? 2 : 1;
-  const int slots = dev.sm_count * per_sm;
-  a.cluster = std::max(1, std::min({8, a.num_kb, slots / std::max(1, tiles * cols)}));
-  const int local = ceil_div(a.num_kb, a.cluster);
-  const uint32_t budget = per_sm == 2 ? 110 * 1024 : 220 * 1024;
-  a.ring = std::max(2, std::min({L::kMaxRing, local, static_cast<int>(budget / L::kStage)}));
-  const size_t smem = std::max<size_t>(a.ring * L::kStage, a.cluster > 1 ? L::kPartial : 0) + L::kMisc + 1024;
-  auto kernel = fp4_rows_kernel<FMT, NT>;
+  const RowsPlan p = plan_rows<FMT, NT, FUSED>(tiles * cols, a.num_kb, dev.sm_count);
+  if (p.smem > dev.max_smem_optin) return ASHQK_ERR_UNSUPPORTED;
+  a.cluster = p.cluster;
+  a.ring = p.ring;
+  a.off_x = p.off_x;
+  a.off_slots = p.off_slots;
+  a.off_bar = p.off_bar;
+  auto kernel = fp4_rows_kernel<FMT, NT, FUSED>;
   static std::atomic<bool> configured[64];  // zero-initialised (static storage)
   if (!configured[dev.device].load(std::memory_order_acquire)) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dev.max_smem_optin)) != cudaSuccess)
@@ -291,7 +456,7 @@ int launch_rows(const RowsMaps& maps, RowsArgs a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(tiles * a.cluster, cols);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = p.smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -306,15 +471,33 @@ int launch_rows(const RowsMaps& maps, RowsArgs a, cudaStream_t stream) {
 }
 
 template <int FMT>
-int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, cudaStream_t stream) {
+int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, bool fused, cudaStream_t stream) {
+  if (fused) return nt == 8 ? launch_rows<FMT, 8, true>(maps, a, stream) : launch_rows<FMT, 16, true>(maps, a, stream);
   switch (nt) {
-    case 8: return launch_rows<FMT, 8>(maps, a, stream);
-    case 16: return launch_rows<FMT, 16>(maps, a, stream);
-    case 32: return launch_rows<FMT, 32>(maps, a, stream);
-    case 64: return launch_rows<FMT, 64>(maps, a, stream);
-    case 128: return launch_rows<FMT, 128>(maps, a, stream);
-    default: return launch_rows<FMT, 256>(maps, a, stream);
+    case 8: return launch_rows<FMT, 8, false>(maps, a, stream);
+    case 16: return launch_rows<FMT, 16, false>(maps, a, stream);
+    case 32: return launch_rows<FMT, 32, false>(maps, a, stream);
+    case 64: return launch_rows<FMT, 64, false>(maps, a, stream);
+    case 128: return launch_rows<FMT, 128, false>(maps, a, stream);
+    default: return launch_rows<FMT, 256, false>(maps, a, stream);
   }
+}
+
+int rows_args(RowsArgs& a, RowsMaps& maps, const void* b_codes, int64_t b_ld, const void* b_scales, void* y, int64_t y_ld,
+              int dtype, int M, int N, int K, int format, float alpha) {
+  a.ws = static_cast<const uint8_t*>(b_scales);
+  a.y = y;
+  a.y_ld = y_ld;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(K), 64));
+  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(K), kFp4BlockK));
+  a.scale_tiles = static_cast<int>(fp4_scale_tiles(K, format));
+  a.alpha = alpha;
+  a.bf16 = dtype == ASHQK_BF16;
+  return encode_tensor_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(b_codes), fp4_padded_k(K) / 2, N, b_ld,
+                              128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 }  // namespace
@@ -325,27 +508,44 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
   int nt = 8;
   while (nt < M && nt < 256) nt *= 2;
   RowsMaps maps;
-  const uint64_t row_bytes = fp4_padded_k(K) / 2;
-  int rc = encode_tensor_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(b_codes), row_bytes, N, b_ld,
-                                128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B);
+  RowsArgs a = {};
+  int rc = rows_args(a, maps, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N, K, format, alpha);
   if (!rc)
-    rc = encode_tensor_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(a_codes), row_bytes, M, a_ld, 128,
-                              nt, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = encode_tensor_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(a_codes), fp4_padded_k(K) / 2, M, a_ld,
+                              128, nt, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc) return rc;
-  RowsArgs a;
-  a.ws = static_cast<const uint8_t*>(b_scales);
   a.xs = static_cast<const uint8_t*>(a_scales);
-  a.y = y;
-  a.y_ld = y_ld;
-  a.M = M;
-  a.N = N;
-  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(K), 64));
-  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(K), kFp4BlockK));
-  a.scale_tiles = static_cast<int>(fp4_scale_tiles(K, format));
-  a.alpha = alpha;
-  a.bf16 = dtype == ASHQK_BF16;
-  return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, stream)
-                               : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, stream);
+  return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, false, stream)
+                               : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, false, stream);
+}
+
+// Whether w4a4_linear quantises x inside the product: up to 16 rows, of a length whose slice fits beside the ring (an
+// eighth of 32768 columns: 16 stages of at most 3 KB).
+bool fp4_fused_ok(int M, int K) { return M <= 16 && K <= 32768; }
+
+int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
+                    const void* w_scales, void* y, int64_t y_ld, int M, int N, int K, int format, float alpha,
+                    cudaStream_t stream) {
+  RowsMaps maps;
+  RowsArgs a = {};
+  const int rc = rows_args(a, maps, w_codes, w_ld, w_scales, y, y_ld, dtype, M, N, K, format, alpha);
+  if (rc) return rc;
+  maps.x = maps.w;  // not used
+  a.x = x;
+  a.x_ld = x_ld;
+  a.x_gs = x_gs;
+  a.gated = gated;
+  a.vec = aligned(x, 16) && x_ld % 8 == 0 && (!gated || K % 8 == 0);
+  const int nt = M <= 8 ? 8 : 16;
+  return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, true, stream)
+                               : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, true, stream);
 }
 
 }  // namespace ashqk
+
+extern "C" int ashqk_fp4_set_tuning(int cluster, int ring) {
+  if (cluster < 0 || cluster > ashqk::kMaxCluster || ring < 0 || ring == 1 || ring > ashqk::kMaxRing) return ASHQK_ERR_INVALID_ARGUMENT;
+  ashqk::g_cluster.store(cluster, std::memory_order_relaxed);
+  ashqk::g_ring.store(ring, std::memory_order_relaxed);
+  return ASHQK_OK;
+}

@@ -18,6 +18,11 @@ int fp4_matmul_pair(const void* a_codes, int64_t a_ld, const void* a_scales, con
                     const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
                     cudaStream_t stream);
 
+bool fp4_fused_ok(int M, int K);
+int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
+                    const void* w_scales, void* y, int64_t y_ld, int M, int N, int K, int format, float alpha,
+                    cudaStream_t stream);
+
 namespace {
 
 std::atomic<int> g_matmul_kernel{0};
@@ -55,7 +60,8 @@ extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a
 extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes) {
   if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   size_t offset;
-  workspace_layout(M, K, format, &offset, bytes);
+  *bytes = 0;
+  if (!fp4_fused_ok(M, K)) workspace_layout(M, K, format, &offset, bytes);
   return ASHQK_OK;
 }
 
@@ -68,6 +74,9 @@ extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gat
   if (!fp4_global_scale_ok(format, x_scale) || !fp4_global_scale_ok(format, w_scale)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(w_codes, w_ld, w_scales, K)) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (fp4_fused_ok(M, K))
+    return fp4_linear_rows(x, x_ld, dtype, gated != 0, x_scale, w_codes, w_ld, w_scales, y, y_ld, M, N, K, format,
+                           x_scale * w_scale, st);
   size_t offset, bytes;
   workspace_layout(M, K, format, &offset, &bytes);
   if (!workspace || workspace_bytes < bytes || !aligned(workspace, 16)) return ASHQK_ERR_WORKSPACE;

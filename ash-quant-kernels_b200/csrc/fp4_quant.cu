@@ -17,7 +17,7 @@ constexpr int kQuantThreads = 256;
 
 template <int FMT, typename T, bool GATED>
 __global__ void __launch_bounds__(kQuantThreads)
-    quantize_fp4_kernel(const T* __restrict__ x, int64_t x_ld, uint8_t* __restrict__ codes, int64_t codes_ld,
+    quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, int64_t codes_ld,
                         uint8_t* __restrict__ scales, int64_t rows, int K, float gs, bool vec, int early) {
   constexpr int kLanes = fp4_block(FMT) / 8;  // lanes of a block
   pdl_wait();
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kQuantThreads)
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(kQuantThreads)
-    dequantize_fp4_kernel(const uint8_t* __restrict__ codes, int64_t codes_ld, const uint8_t* __restrict__ scales,
+    dequantize_fp4_kernel(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales,
                           T* __restrict__ out, int64_t out_ld, int64_t rows, int K, float gs, bool vec) {
   pdl_wait();
   const int chunks = (K + 7) / 8;

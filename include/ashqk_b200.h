@@ -377,6 +377,12 @@ ASHQK_API int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gate
  */
 ASHQK_API int ashqk_set_fp4_kernel(int which);
 
+/*
+ * The same for the rows kernel's plan: CTAs per cluster (up to 8) and stages in flight (2 to 12) instead of the
+ * automatic ones; 0 restores them.
+ */
+ASHQK_API int ashqk_fp4_set_tuning(int cluster, int ring);
+
 #ifdef __cplusplus
 }
 #endif

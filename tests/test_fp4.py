@@ -140,6 +140,14 @@ def test_c_abi_sizes():
         assert lib.ashqk_w4a4_workspace_size(m, n_, k, fmt, ctypes.byref(size)) == 1
 
 
+def test_c_abi_switches():
+    lib = _lib()
+    for which, want in ((0, 0), (1, 0), (2, 0), (3, 1), (-1, 1), (0, 0)):
+        assert lib.ashqk_set_fp4_kernel(which) == want
+    for cluster, ring, want in ((1, 2, 0), (8, 12, 0), (9, 2, 1), (-1, 0, 1), (0, 1, 1), (0, 13, 1), (0, -1, 1), (0, 0, 0)):
+        assert lib.ashqk_fp4_set_tuning(cluster, ring) == want
+
+
 def _refusals(good: dict, bad: list):
     """Each bad change alone must be refused as an invalid argument."""
     for change in bad:

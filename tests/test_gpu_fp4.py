@@ -291,6 +291,32 @@ def test_same_result_every_time(fmt, m):
         assert torch.equal(ashqk.w4a4_linear(x, w, global_scale=G[fmt]), first)
 
 
+@pytest.mark.parametrize("cluster", [1, 2, 3, 5, 8])
+@pytest.mark.parametrize("ring", [2, 3, 7])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_every_split_of_k(cluster, ring, fmt):
+    """The rows kernel's plans: clusters that divide K evenly and not, rings shorter than a CTA's slice, every
+    instruction width, sums in shared memory of their own and in the ring's."""
+    import ctypes
+
+    from ashqk import _ext
+
+    lib = ctypes.CDLL(_ext.C_LIBRARY)
+    assert lib.ashqk_fp4_set_tuning(cluster, ring) == 0 and lib.ashqk_set_fp4_kernel(1) == 0
+    try:
+        for m, n, k in ((1, 300, 2080), (4, 128, 4096), (13, 256, 1500), (30, 200, 2304), (61, 130, 1024), (100, 128, 2080), (200, 256, 1056), (300, 140, 800)):
+            b, b64 = random_operand(n, k, fmt, n)
+            a, a64 = random_operand(m, k, fmt, m)
+            check_product(ashqk.fp4_matmul(a, b), a64, b64)
+            if m <= 16:
+                x = rows(m, k, "bf16", m, spread=False)
+                code, byte = F.quantize(x.double().cpu().numpy(), fmt, G[fmt])
+                x64 = torch.from_numpy(F.values(code, byte, fmt, G[fmt])[:, :k]).cuda()
+                check_product(ashqk.w4a4_linear(x, b, global_scale=G[fmt]), x64, b64, 2.0**-23)
+    finally:
+        assert lib.ashqk_fp4_set_tuning(0, 0) == 0 and lib.ashqk_set_fp4_kernel(0) == 0
+
+
 def test_empty():
     w, _ = random_operand(64, 96, "mxfp4", 1)
     assert ashqk.w4a4_linear(torch.zeros(0, 96, dtype=torch.float16, device="cuda"), w).shape == (0, 64)
