@@ -16,6 +16,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace ashqk {
@@ -34,37 +36,54 @@ __device__ __forceinline__ int64_t fp4_scale_offset(int64_t row, int block, int6
   return ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
-// The scale of a block whose largest magnitude has the fp32 bit pattern `amax` (sign cleared): its
-// byte, and through `*divisor` what the block's values are divided by. A block that holds an infinity
-// or a NaN (the pattern compares above every finite one) gets the format's NaN scale.
+// What a quantiser needs of the global scale g; on the host.
+struct Fp4Quant {
+  float gs, six_gs, inv_six_gs;  // g, 6 g and 1 / (6 g), each rounded to fp32
+};
+inline Fp4Quant fp4_quant_params(float gs) {
+  const float six = 6.0f * gs;
+  return {gs, six, 1.0f / six};
+}
+
+// v / d, rounded to fp32 as one division is, from r = 1 / d correctly rounded: the product v r is off by at most a
+// unit in the last place, and one step with the exact residual corrects it (P. W. Markstein, Computation of
+// elementary functions on the IBM RISC System/6000 processor, IBM J. Res. Dev. 34, 1990). Quotients are cut
+// off at +-1024, beyond what either format holds, so that the residual stays finite.
+__device__ __forceinline__ float quotient(float v, float d, float r) {
+  const float q = fminf(fmaxf(v * r, -1024.0f), 1024.0f);
+  return fmaf(fmaf(-q, d, v), r, q);
+}
+
+// The scale of a block whose largest magnitude has the fp32 bit pattern `amax` (sign cleared): its byte, its value d
+// and 1 / d. A block that holds an infinity or a NaN (the pattern compares above every finite one) gets the
+// format's NaN scale. A scale of zero (NVFP4, a tiny block) comes with a reciprocal of zero.
 template <int FMT>
-__device__ __forceinline__ uint32_t fp4_scale_of(uint32_t amax, float gs, float* divisor) {
+__device__ __forceinline__ uint32_t fp4_scale_of(uint32_t amax, const Fp4Quant& q, float* d, float* r) {
   if (FMT == ASHQK_MXFP4) {
-    // Exponent field E of amax; the scale's is E - 2, not below 0 (2^-127).
+    // Exponent field E of amax; the scale's is E - 2, not below 0 (2^-127). Its inverse 2^(127 - byte) is exact.
     const uint32_t e = amax >> 23;
     const uint32_t byte = amax >= 0x7f800000u ? 255u : (e > 2u ? e - 2u : 0u);
-    // Its inverse 2^(127 - byte), exact: the "division" is a multiplication.
-    *divisor = __uint_as_float((254u - (byte == 255u ? 254u : byte)) << 23);
+    *d = 0.0f;  // not used
+    *r = __uint_as_float((254u - (byte == 255u ? 254u : byte)) << 23);
     return byte;
   } else {
-    const float t = __fdiv_rn(__uint_as_float(amax), 6.0f * gs);
+    const float t = quotient(__uint_as_float(amax), q.six_gs, q.inv_six_gs);
     uint16_t pair;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(pair) : "f"(0.0f), "f"(t));
     const uint32_t byte = amax >= 0x7f800000u ? 0x7fu : (pair & 0x7fu);
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
-    *divisor = __low2float(u32_as_h2(h2)) * gs;
+    *d = __low2float(u32_as_h2(h2)) * q.gs;
+    *r = *d > 0.0f ? __frcp_rn(*d) : 0.0f;
     return byte;
   }
 }
 
-// A value over its scale, before rounding to E2M1.
+// A value over its scale, before rounding to E2M1. For NVFP4 the rounded quotient and not the product with the
+// reciprocal, which would move exact ties (x = 0.75 d, which 16-bit inputs meet often) off the border.
 template <int FMT>
-__device__ __forceinline__ float fp4_scaled(float v, float divisor) {
-  if (FMT == ASHQK_MXFP4) return v * divisor;
-  // The rounded quotient: a product with the reciprocal would move exact ties (x = 0.75 S, which 16-bit
-  // inputs meet often) off the border. Zero for a scale that rounded to zero.
-  return divisor > 0.0f ? __fdiv_rn(v, divisor) : 0.0f;
+__device__ __forceinline__ float fp4_scaled(float v, float d, float r) {
+  return FMT == ASHQK_MXFP4 ? v * r : quotient(v, d, r);
 }
 
 // Eight scaled values -> eight E2M1 codes, the first in the lowest four bits; to nearest even, held
@@ -173,31 +192,55 @@ __device__ __forceinline__ uint4 ld_once_v4(const void* p) {
   return v;
 }
 
-// Eight consecutive values: `vec` when p is 16-byte aligned and all eight exist, else one by one with
-// zeros from `count` on.
+// Eight consecutive 16-bit values as they lie in memory: `vec` when p is 16-byte aligned and all eight exist, else
+// one by one with zeros from `count` on.
+template <typename T>
+__device__ __forceinline__ uint4 load8_raw(const T* p, int count, bool vec) {
+  static_assert(sizeof(T) == 2, "16-bit types");
+  if (vec) return ld_once_v4(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
+    w[i] = (2 * i < count ? h[0] : 0u) | ((2 * i + 1 < count ? h[1] : 0u) << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  unpack2<T>(u.x, v[0], v[1]);
+  unpack2<T>(u.y, v[2], v[3]);
+  unpack2<T>(u.z, v[4], v[5]);
+  unpack2<T>(u.w, v[6], v[7]);
+}
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
-  if (vec) {
-    if (sizeof(T) == 2) {
-      const uint4 u = ld_once_v4(p);
-      unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.x, v[0], v[1]);
-      unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.y, v[2], v[3]);
-      unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.z, v[4], v[5]);
-      unpack2<std::conditional_t<sizeof(T) == 2, T, __half>>(u.w, v[6], v[7]);
-    } else {
-      const uint4 a = ld_once_v4(p), b = ld_once_v4(p + 4);
-      v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-      v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-    }
+  if constexpr (sizeof(T) == 2) {
+    unpack8<T>(load8_raw(p, count, vec), v);
+  } else if (vec) {
+    const uint4 a = ld_once_v4(p), b = ld_once_v4(p + 4);
+    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? to_f32<T>(p[i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = i < count ? p[i] : 0.0f;
   }
 }
 
 // silu(gate) * up in fp32. exp overflows to infinity for gates below -88 and the quotient is then 0.
 __device__ __forceinline__ float silu_mul(float gate, float up) {
   return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+}
+
+// The largest magnitude of eight 16-bit values, as the fp32 bit pattern of its absolute value.
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max8_raw(const uint4& u) {
+  uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
+  m = max(m & 0xffffu, m >> 16);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    return m << 16;
+  else
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
 }
 
 // The largest bit pattern of |v|: as an unsigned number it orders finite < infinity < NaN.

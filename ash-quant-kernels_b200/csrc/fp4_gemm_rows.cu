@@ -46,7 +46,8 @@ struct RowsArgs {
   int M, N, K, k_steps, num_kb, scale_tiles;  // k_steps: MMAs of 64 columns over all of K
   int cluster, ring;
   uint32_t off_x, off_slots, off_bar;  // shared memory after the ring
-  float alpha, x_gs;
+  float alpha;
+  Fp4Quant xq;
   int bf16, gated, vec;
 };
 
@@ -95,50 +96,69 @@ __device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
 }
 
 // Quantises columns [256 kb0, 256 kb1) of A's rows into shared memory. Eight columns per thread, a block's
-// lanes adjacent, as in the quantiser proper.
-template <int FMT, int NT, typename T>
+// lanes adjacent, as in the quantiser proper; two chunks' loads in flight.
+template <int FMT, int NT, typename T, bool GATED>
 __device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int kb1, uint32_t codes, uint32_t scales, int tid) {
   using L = RowsShape<FMT, NT, true>;
   constexpr int kLanes = fp4_block(FMT) / 8;
-  const int chunks = (kb1 - kb0) * 32;
-  const int total = a.M * chunks;  // a multiple of 32: warps stay whole
+  constexpr int kBatch = 2;
+  constexpr int kStep = 32 * kQuantWarps;
+  const int chunks = (kb1 - kb0) * 32;  // of a row: a multiple of 32, so that warps stay in one row
   const T* x = static_cast<const T*>(a.x);
-  for (int i = tid; i < total; i += 32 * kQuantWarps) {
-    const int m = i / chunks;
-    const int c = i - m * chunks;
-    const int k0 = kb0 * kFp4BlockK + c * 8;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (k0 < a.K) {
-      const T* p = x + m * a.x_ld + k0;
-      const bool whole = a.vec && k0 + 8 <= a.K;
-      load8<T>(p, a.K - k0, whole, v);
-      if (a.gated) {
-        float u[8];
-        load8<T>(p + a.K, a.K - k0, whole, u);
+  int m = 0, c = tid;  // row and chunk
+  while (c >= chunks) c -= chunks, ++m;
+  while (m < a.M) {
+    uint4 g[kBatch], u[kBatch];
+    int bm[kBatch], bc[kBatch];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
+    for (int b = 0; b < kBatch; ++b) {
+      bm[b] = m, bc[b] = c;
+      g[b] = u[b] = make_uint4(0, 0, 0, 0);
+      const int k0 = kb0 * kFp4BlockK + c * 8;
+      if (m < a.M && k0 < a.K) {
+        const T* p = x + m * a.x_ld + k0;
+        const bool whole = a.vec && k0 + 8 <= a.K;
+        g[b] = load8_raw(p, a.K - k0, whole);
+        if (GATED) u[b] = load8_raw(p + a.K, a.K - k0, whole);
       }
+      c += kStep;
+      while (c >= chunks) c -= chunks, ++m;
     }
-    uint32_t amax = abs_max8(v);
 #pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    float divisor;
-    const uint32_t byte = fp4_scale_of<FMT>(amax, a.x_gs, &divisor);
+    for (int b = 0; b < kBatch; ++b) {
+      if (bm[b] >= a.M) break;  // whole warps
+      float v[8];
+      unpack8<T>(g[b], v);
+      uint32_t amax;
+      if (GATED) {
+        float w[8];
+        unpack8<T>(u[b], w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], divisor);
-    const int kb = c >> 5, cc = c & 31;
-    const uint32_t at = codes + kb * L::kX + (m >> 3) * 1024 + (m & 7) * 128 + (((cc >> 2) ^ (m & 7)) << 4) + (cc & 3) * 4;
-    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(fp4_pack8(v)) : "memory");
-    if (cc % kLanes == 0) {
-      const int block = cc / kLanes;
-      const uint32_t s = scales + (kb * L::kT + (block >> 2)) * L::kXSTile + m * 16 + (block & 3);
-      asm volatile("st.shared.u8 [%0], %1;" ::"r"(s), "r"(byte) : "memory");
+        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], w[j]);
+        amax = abs_max8(v);
+      } else {
+        amax = abs_max8_raw<T>(g[b]);
+      }
+#pragma unroll
+      for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+      float d, r;
+      const uint32_t byte = fp4_scale_of<FMT>(amax, a.xq, &d, &r);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], d, r);
+      const int row = bm[b], kb = bc[b] >> 5, cc = bc[b] & 31;
+      const uint32_t at = codes + kb * L::kX + (row >> 3) * 1024 + (row & 7) * 128 + (((cc >> 2) ^ (row & 7)) << 4) + (cc & 3) * 4;
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(fp4_pack8(v)) : "memory");
+      if (cc % kLanes == 0) {
+        const int block = cc / kLanes;
+        const uint32_t s = scales + (kb * L::kT + (block >> 2)) * L::kXSTile + row * 16 + (block & 3);
+        asm volatile("st.shared.u8 [%0], %1;" ::"r"(s), "r"(byte) : "memory");
+      }
     }
   }
 }
 
 template <int FMT, int NT, bool FUSED>
-__global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_constant__ RowsMaps maps, const RowsArgs a) {
   using L = RowsShape<FMT, NT, FUSED>;
   using Mma = Fp4Mma<FMT>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -301,10 +321,17 @@ __global__ void __launch_bounds__(kThreads) fp4_rows_kernel(const __grid_constan
     mbar_drain(done, 0);
   } else if (FUSED) {
     const int tid = static_cast<int>(threadIdx.x) - 64;
-    if (a.bf16)
-      quantize_slice<FMT, NT, __nv_bfloat16>(a, kb0, kb1, x_codes, x_scales, tid);
-    else
-      quantize_slice<FMT, NT, __half>(a, kb0, kb1, x_codes, x_scales, tid);
+    if (a.gated) {
+      if (a.bf16)
+        quantize_slice<FMT, NT, __nv_bfloat16, true>(a, kb0, kb1, x_codes, x_scales, tid);
+      else
+        quantize_slice<FMT, NT, __half, true>(a, kb0, kb1, x_codes, x_scales, tid);
+    } else {
+      if (a.bf16)
+        quantize_slice<FMT, NT, __nv_bfloat16, false>(a, kb0, kb1, x_codes, x_scales, tid);
+      else
+        quantize_slice<FMT, NT, __half, false>(a, kb0, kb1, x_codes, x_scales, tid);
+    }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(x_ready);
@@ -533,7 +560,7 @@ int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_
   maps.x = maps.w;  // not used
   a.x = x;
   a.x_ld = x_ld;
-  a.x_gs = x_gs;
+  a.xq = fp4_quant_params(x_gs);
   a.gated = gated;
   a.vec = aligned(x, 16) && x_ld % 8 == 0 && (!gated || K % 8 == 0);
   const int nt = M <= 8 ? 8 : 16;

@@ -1,11 +1,11 @@
 // Quantising rows to microscaled 4-bit floating point, plain or of silu(gate) * up, and reading
 // them back.
 //
-// One thread takes eight columns (16 bytes of a 16-bit input, 4 bytes of codes); the lanes of a block
+// One thread takes chunks of eight columns (16 bytes of a 16-bit input, 4 bytes of codes); the lanes of a block
 // (4 for MXFP4, 2 for NVFP4) share its largest magnitude by shuffles, so every value is read once and
 // nothing passes through shared memory. HBM-bound: a value costs its input, half a byte of code and
-// 1/32 or 1/16 byte of scale.
-#include <type_traits>
+// 1/32 or 1/16 byte of scale. Where there are enough chunks a thread takes four, their loads in flight together.
+#include <algorithm>
 
 #include "fp4.cuh"
 #include "sm100.cuh"
@@ -15,81 +15,148 @@ namespace {
 
 constexpr int kQuantThreads = 256;
 
-template <int FMT, typename T, bool GATED>
+// i / d for i < 2^31 by a multiplication: m = ceil(2^(31 + s) / d) with 2^(s-1) < d <= 2^s has an error small enough
+// for 31-bit numerators (T. Granlund, P. L. Montgomery, Division by invariant integers using
+// multiplication, 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) ++s;
+  return {d, static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), s};
+}
+__device__ __forceinline__ uint32_t divide(uint32_t i, const FastDiv& f) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(i) * f.mul) >> (31 + f.shift));
+}
+
+// WHOLE: every row is whole tiles of four blocks, whose scales then leave as one 4-byte store.
+template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, int64_t codes_ld,
-                        uint8_t* __restrict__ scales, int64_t rows, int K, float gs, bool vec, int early) {
+                        uint8_t* __restrict__ scales, int64_t row0, uint32_t total, int K, FastDiv by_chunks, Fp4Quant q,
+                        bool vec, int early) {
   constexpr int kLanes = fp4_block(FMT) / 8;  // lanes of a block
   pdl_wait();
   if (early) pdl_launch_dependents();
-  const int chunks = static_cast<int>(fp4_padded_k(K) / 8);  // a multiple of 4: a block's lanes share a row
+  const uint32_t chunks = by_chunks.d;  // of a row; a multiple of 4: a block's lanes share a row
   const int64_t tiles = fp4_scale_tiles(K, FMT);
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-  const bool live = idx < rows * chunks;
-  const int64_t row = live ? idx / chunks : 0;
-  const int chunk = live ? static_cast<int>(idx - row * chunks) : 0;
-  const int k0 = chunk * 8;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live && k0 < K) {
-    const T* p = x + row * x_ld + k0;
-    const bool whole = vec && k0 + 8 <= K;
-    load8<T>(p, K - k0, whole, v);
-    if (GATED) {
-      float u[8];
-      load8<T>(p + K, K - k0, whole, u);
+  const uint32_t first = blockIdx.x * (kQuantThreads * BATCH) + threadIdx.x;
+  uint4 g[BATCH], u[BATCH];
+  float gf[sizeof(T) == 4 ? BATCH : 1][8], uf[sizeof(T) == 4 ? BATCH : 1][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = silu_mul(v[i], u[i]);
+  for (int b = 0; b < BATCH; ++b) {
+    const uint32_t i = first + b * kQuantThreads;
+    const uint32_t r = divide(i, by_chunks);
+    const int k0 = static_cast<int>(i - r * chunks) * 8;
+    const bool live = i < total && k0 < K;
+    const T* p = x + (row0 + r) * x_ld + k0;
+    const bool whole = vec && k0 + 8 <= K;
+    if constexpr (sizeof(T) == 2) {
+      g[b] = u[b] = make_uint4(0, 0, 0, 0);
+      if (live) g[b] = load8_raw(p, K - k0, whole);
+      if (live && GATED) u[b] = load8_raw(p + K, K - k0, whole);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) gf[b][j] = uf[b][j] = 0.0f;
+      if (live) load8<T>(p, K - k0, whole, gf[b]);
+      if (live && GATED) load8<T>(p + K, K - k0, whole, uf[b]);
     }
   }
-  uint32_t amax = abs_max8(v);
 #pragma unroll
-  for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-  if (!live) return;
-  float divisor;
-  const uint32_t byte = fp4_scale_of<FMT>(amax, gs, &divisor);
+  for (int b = 0; b < BATCH; ++b) {
+    const uint32_t i = first + b * kQuantThreads;
+    float v[8], w[8];
+    uint32_t amax;
+    if constexpr (sizeof(T) == 2) {
+      unpack8<T>(g[b], v);
+      if (GATED) unpack8<T>(u[b], w);
+    } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = fp4_scaled<FMT>(v[i], divisor);
-  *reinterpret_cast<uint32_t*>(codes + row * codes_ld + chunk * 4) = fp4_pack8(v);
-  if (chunk % kLanes == 0) {
-    const int block = chunk / kLanes;
+      for (int j = 0; j < 8; ++j) v[j] = gf[b][j], w[j] = uf[b][j];
+    }
+    if constexpr (GATED) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], w[j]);
+      amax = abs_max8(v);
+    } else if constexpr (sizeof(T) == 2) {
+      amax = abs_max8_raw<T>(g[b]);
+    } else {
+      amax = abs_max8(v);
+    }
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    float d, r;
+    uint32_t bytes = fp4_scale_of<FMT>(amax, q, &d, &r);
+    const uint32_t rr = divide(i, by_chunks);
+    const uint32_t chunk = i - rr * chunks;
+    const int64_t row = row0 + rr;
+    const int block = static_cast<int>(chunk / kLanes);
+    if (WHOLE) {
+      bytes <<= 8 * (block & 3);
+      bytes |= __shfl_xor_sync(0xffffffffu, bytes, kLanes);
+      bytes |= __shfl_xor_sync(0xffffffffu, bytes, 2 * kLanes);
+    }
+    if (i >= total) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], d, r);
+    *reinterpret_cast<uint32_t*>(codes + row * codes_ld + chunk * 4) = fp4_pack8(v);
     uint8_t* s = scales + fp4_scale_offset(row, block, tiles);
-    *s = static_cast<uint8_t>(byte);
-    if (block == chunks / kLanes - 1)  // the tile's padding blocks
-      for (int b = block + 1; b & 3; ++b) *++s = 0;
+    if (WHOLE) {
+      if (chunk % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
+    } else if (chunk % kLanes == 0) {
+      *s = static_cast<uint8_t>(bytes);
+      if (chunk + kLanes == chunks)  // the tile's padding blocks
+        for (int k = block + 1; k & 3; ++k) *++s = 0;
+    }
   }
 }
 
-template <int FMT, typename T>
+template <int FMT, typename T, int BATCH>
 __global__ void __launch_bounds__(kQuantThreads)
-    dequantize_fp4_kernel(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales,
-                          T* __restrict__ out, int64_t out_ld, int64_t rows, int K, float gs, bool vec) {
+    dequantize_fp4_kernel(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, T* __restrict__ out,
+                          int64_t out_ld, int64_t row0, uint32_t total, int K, FastDiv by_chunks, float gs, bool vec) {
   pdl_wait();
-  const int chunks = (K + 7) / 8;
+  const uint32_t chunks = by_chunks.d;
   const int64_t tiles = fp4_scale_tiles(K, FMT);
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kQuantThreads + threadIdx.x;
-  if (idx >= rows * chunks) return;
-  const int64_t row = idx / chunks;
-  const int chunk = static_cast<int>(idx - row * chunks);
-  const int k0 = chunk * 8;
-  float v[8];
-  fp4_unpack8(*reinterpret_cast<const uint32_t*>(codes + row * codes_ld + chunk * 4), v);
-  const float s = fp4_scale_value<FMT>(scales[fp4_scale_offset(row, k0 / fp4_block(FMT), tiles)]);
+  const uint32_t first = blockIdx.x * (kQuantThreads * BATCH) + threadIdx.x;
+  uint32_t c[BATCH], s[BATCH];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = v[i] * s * gs;
-  T* o = out + row * out_ld + k0;
-  if (vec && k0 + 8 <= K) {
-    if (sizeof(T) == 2) {
-      using H = std::conditional_t<sizeof(T) == 2, T, __half>;
-      *reinterpret_cast<uint4*>(o) =
-          make_uint4(pack2<H>(v[0], v[1]), pack2<H>(v[2], v[3]), pack2<H>(v[4], v[5]), pack2<H>(v[6], v[7]));
-    } else {
-      reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-      reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  for (int b = 0; b < BATCH; ++b) {
+    const uint32_t i = first + b * kQuantThreads;
+    const uint32_t r = divide(i, by_chunks);
+    const uint32_t chunk = i - r * chunks;
+    c[b] = s[b] = 0;
+    if (i < total) {
+      c[b] = *reinterpret_cast<const uint32_t*>(codes + (row0 + r) * codes_ld + chunk * 4);
+      s[b] = scales[fp4_scale_offset(row0 + r, static_cast<int>(chunk * 8 / fp4_block(FMT)), tiles)];
     }
-  } else {
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (k0 + i < K) o[i] = from_f32<T>(v[i]);
+  for (int b = 0; b < BATCH; ++b) {
+    const uint32_t i = first + b * kQuantThreads;
+    if (i >= total) break;
+    const uint32_t r = divide(i, by_chunks);
+    const int k0 = static_cast<int>(i - r * chunks) * 8;
+    float v[8];
+    fp4_unpack8(c[b], v);
+    const float sv = fp4_scale_value<FMT>(s[b]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * sv * gs;
+    T* o = out + (row0 + r) * out_ld + k0;
+    if (vec && k0 + 8 <= K) {
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(o) =
+            make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+      } else {
+        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k0 + j < K) o[j] = from_f32<T>(v[j]);
+    }
   }
 }
 
@@ -108,25 +175,62 @@ int launch_pdl(void (*kernel)(Params...), int64_t blocks, int threads, cudaStrea
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) == cudaSuccess ? ASHQK_OK : ASHQK_ERR_CUDA;
 }
 
+constexpr int kBatch = 4;
+// From here on four chunks per thread still leave every SM two blocks (148 SMs).
+constexpr int64_t kBatchChunks = 2 * 148 * kQuantThreads * kBatch;
+
+// Calls launch(row0, chunks, blocks of kQuantThreads * batch) for slabs of rows with fewer than 2^31 chunks.
+template <typename F>
+int for_slabs(int64_t rows, int64_t chunks, int batch, F launch) {
+  const int64_t most = std::max<int64_t>(1, ((1ll << 31) - 2 * kQuantThreads * kBatch) / chunks);
+  for (int64_t row0 = 0; row0 < rows; row0 += most) {
+    const int64_t total = std::min(most, rows - row0) * chunks;
+    if (const int rc = launch(row0, static_cast<uint32_t>(total), ceil_div64(total, kQuantThreads * batch))) return rc;
+  }
+  return ASHQK_OK;
+}
+
+template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
+int quantize_launch(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
+                    bool early, cudaStream_t stream) {
+  const bool vec = aligned(x, 16) && (x_ld * sizeof(T)) % 16 == 0 && (!GATED || (K * sizeof(T)) % 16 == 0);
+  const int64_t chunks = fp4_padded_k(K) / 8;
+  return for_slabs(M, chunks, BATCH, [&](int64_t row0, uint32_t total, int64_t blocks) {
+    return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, BATCH, WHOLE>, blocks, kQuantThreads, stream,
+                      static_cast<const T*>(x), x_ld, codes, codes_ld, scales, row0, total, K,
+                      fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(gs), vec, early);
+  });
+}
+
+template <int FMT, typename T, bool GATED>
+int quantize_shaped(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
+                    bool early, cudaStream_t stream) {
+  const int64_t kp = fp4_padded_k(K);
+  const bool whole = kp % (4 * fp4_block(FMT)) == 0;
+  const bool many = M * (kp / 8) >= kBatchChunks;
+  return (whole ? many ? quantize_launch<FMT, T, GATED, kBatch, true> : quantize_launch<FMT, T, GATED, 1, true>
+          : many ? quantize_launch<FMT, T, GATED, kBatch, false>
+                 : quantize_launch<FMT, T, GATED, 1, false>)(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
+}
+
 template <int FMT, typename T>
 int quantize_typed(const void* x, int64_t x_ld, bool gated, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M,
                    int K, float gs, bool early, cudaStream_t stream) {
-  const bool vec = aligned(x, 16) && (x_ld * sizeof(T)) % 16 == 0 && (!gated || (K * sizeof(T)) % 16 == 0);
-  const int64_t blocks = ceil_div64(M * (fp4_padded_k(K) / 8), kQuantThreads);
-  const T* xt = static_cast<const T*>(x);
-  return gated ? launch_pdl(quantize_fp4_kernel<FMT, T, true>, blocks, kQuantThreads, stream, xt, x_ld, codes,
-                            codes_ld, scales, M, K, gs, vec, early)
-               : launch_pdl(quantize_fp4_kernel<FMT, T, false>, blocks, kQuantThreads, stream, xt, x_ld, codes,
-                            codes_ld, scales, M, K, gs, vec, early);
+  return gated ? quantize_shaped<FMT, T, true>(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream)
+               : quantize_shaped<FMT, T, false>(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
 }
 
 template <int FMT, typename T>
 int dequantize_typed(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, void* out, int64_t out_ld, int M,
                      int K, float gs, cudaStream_t stream) {
   const bool vec = aligned(out, 16) && (out_ld * sizeof(T)) % 16 == 0;
-  const int64_t blocks = ceil_div64(static_cast<int64_t>(M) * ((K + 7) / 8), kQuantThreads);
-  return launch_pdl(dequantize_fp4_kernel<FMT, T>, blocks, kQuantThreads, stream, codes, codes_ld, scales,
-                    static_cast<T*>(out), out_ld, M, K, gs, vec);
+  const int64_t chunks = (K + 7) / 8;
+  const bool many = M * chunks >= kBatchChunks;
+  return for_slabs(M, chunks, many ? kBatch : 1, [&](int64_t row0, uint32_t total, int64_t blocks) {
+    return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kBatch> : dequantize_fp4_kernel<FMT, T, 1>, blocks,
+                      kQuantThreads, stream, codes, codes_ld, scales, static_cast<T*>(out), out_ld, row0, total, K,
+                      fast_div(static_cast<uint32_t>(chunks)), gs, vec);
+  });
 }
 
 }  // namespace
