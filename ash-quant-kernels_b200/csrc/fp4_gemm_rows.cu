@@ -12,7 +12,7 @@
 //               bulk copies of scale tiles
 //   warp 1      one elected lane: tcgen05.cp of a stage's scales, its four MMAs, commit
 //   warps 2..9  fused form: quantise this CTA's slice of A into shared memory, in the layout in which TMA and
-//               the scale tiles arrive otherwise; then warps 2..5: TMEM -> registers -> y, or, with a split K,
+//               the scale tiles arrive otherwise; then all: TMEM -> registers -> y, or, with a split K,
 //               -> the shared memory of the CTA that adds these rows of A (st.async, counted in bytes on
 //               its barrier)
 //
@@ -337,8 +337,9 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     if (lane == 0) mbar_arrive(x_ready);
   }
 
-  // ---- sums: warps 2..5, one lane per weight row ----
-  const bool epilogue = warp >= 2 && warp < 6;
+  // ---- sums: warps 2..9, one lane per weight row; the two warps of a lane quarter take turns ----
+  const bool epilogue = warp >= 2;
+  const int turn = (warp - 2) >> 2;
   const int row = 32 * (warp & 3) + lane;
   const int n = n0 + row;
   bool ok = false;
@@ -355,33 +356,42 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     }
   }
   const uint32_t slots = sbase + (L::kOwnSlots ? a.off_slots : 0u);
-  auto store = [&](int m, float v) {
-    if (m >= a.M || n >= a.N) return;
-    if (a.bf16)
-      static_cast<__nv_bfloat16*>(a.y)[m * a.y_ld + n] = __float2bfloat16_rn(v * a.alpha);
-    else
-      static_cast<__half*>(a.y)[m * a.y_ld + n] = __float2half_rn(v * a.alpha);
+  // Four sums of consecutive rows of A -> y. Lanes are consecutive columns of y: 64 bytes per row and warp.
+  auto store4 = [&](int m, float v0, float v1, float v2, float v3) {
+    if (n >= a.N) return;
+    uint16_t* y = static_cast<uint16_t*>(a.y) + m * a.y_ld + n;
+    const uint32_t lo = a.bf16 ? pack2<__nv_bfloat16>(v0 * a.alpha, v1 * a.alpha) : pack2<__half>(v0 * a.alpha, v1 * a.alpha);
+    const uint32_t hi = a.bf16 ? pack2<__nv_bfloat16>(v2 * a.alpha, v3 * a.alpha) : pack2<__half>(v2 * a.alpha, v3 * a.alpha);
+    if (m < a.M) y[0] = static_cast<uint16_t>(lo);
+    if (m + 1 < a.M) y[a.y_ld] = static_cast<uint16_t>(lo >> 16);
+    if (m + 2 < a.M) y[2 * a.y_ld] = static_cast<uint16_t>(hi);
+    if (m + 3 < a.M) y[3 * a.y_ld] = static_cast<uint16_t>(hi >> 16);
   };
   if (epilogue) {
+    constexpr int kCols = NT < 32 ? 8 : 32;  // columns of one TMEM load
     const uint32_t taddr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
 #pragma unroll 1
-    for (int g = 0; g < groups; g += 2) {
-      uint32_t r[8];
-      tmem_ld_32x32b_x8(taddr + 4 * g, r);
+    for (int g0 = turn * (kCols / 4); g0 < groups; g0 += 2 * (kCols / 4)) {
+      uint32_t r[kCols];
+      if constexpr (kCols == 8)
+        tmem_ld_32x32b_x8(taddr + 4 * g0, r);
+      else
+        tmem_ld_32x32b_x32(taddr + 4 * g0, r);
       tmem_wait_ld();
       if (!ok) {  // a wait ran out: the sums are not there; peers still get the bytes that they count
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = 0x7fffffffu;
+        for (int i = 0; i < kCols; ++i) r[i] = 0x7fffffffu;
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (g + h >= groups) break;
+      for (int h = 0; h < kCols / 4; ++h) {
+        const int g = g0 + h;
+        if (g >= groups) break;
         if (C == 1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) store(m0 + 4 * (g + h) + i, __uint_as_float(r[4 * h + i]));
+          store4(m0 + 4 * g, __uint_as_float(r[4 * h]), __uint_as_float(r[4 * h + 1]), __uint_as_float(r[4 * h + 2]),
+                 __uint_as_float(r[4 * h + 3]));
         } else {
-          const int owner = (g + h) % C;
-          const uint32_t at = slots + static_cast<uint32_t>((((g + h) / C) * C + rank) * kTileN + row) * 16;
+          const int l = g / C, owner = g - l * C;
+          const uint32_t at = slots + static_cast<uint32_t>((l * C + rank) * kTileN + row) * 16;
           uint32_t remote, bar;
           asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(owner));
           asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(received)), "r"(owner));
@@ -401,15 +411,15 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     __syncwarp();
     cluster_arrive();
     if (epilogue && my_groups > 0 && mbar_wait_cluster(received, 0, abort)) {
-#pragma unroll 1
-      for (int l = 0; l < my_groups; ++l) {
+#pragma unroll 2
+      for (int l = turn; l < my_groups; l += 2) {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int c = 0; c < C; ++c) {
           const uint4 p = lds_v4(slots + static_cast<uint32_t>((l * C + c) * kTileN + row) * 16);
           s[0] += __uint_as_float(p.x), s[1] += __uint_as_float(p.y), s[2] += __uint_as_float(p.z), s[3] += __uint_as_float(p.w);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) store(m0 + 4 * (l * C + rank) + i, s[i]);
+        store4(m0 + 4 * (l * C + rank), s[0], s[1], s[2], s[3]);
       }
     }
     __syncwarp();
@@ -425,13 +435,20 @@ struct RowsPlan {
   uint32_t off_x, off_slots, off_bar, smem;
 };
 
-// CTAs per cluster and stages in flight for `tiles` tiles of 128 weight rows (times the row blocks of A).
+// CTAs per cluster and stages in flight for `tiles` tiles of 128 weight rows (times the row blocks of A). Measured at
+// one to 128 rows on layers of 32 to 192 tiles, every cluster size and ring, launches back to back in a
+// graph. What a split saves is a CTA's serial run over its stages (0.27 us each); what it costs, beyond 1.35 CTAs
+// per SM, is the room in which the next launch's CTAs start early: 32 tiles at one row 8.0 us with one CTA
+// per cluster, 4.5 with 4 to 6, 5.8 with 7; 48 tiles 8.0, 5.0 with 4, 6.3 with 6. With more tiles than SMs a
+// split in two evens out the last wave (192 tiles: 13.4 -> 12.5 us).
 template <int FMT, int NT, bool FUSED>
 RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   using L = RowsShape<FMT, NT, FUSED>;
   RowsPlan p;
-  const int per_sm = L::kTmemCols <= 256 ? 2 : 1;
-  p.cluster = std::max(1, std::min({kMaxCluster, num_kb, sm_count * per_sm / std::max(1, tiles)}));
+  // Wide tiles without slots of their own have an SM to themselves, and clusters of such CTAs do not fill every SM.
+  const int ctas = L::kTmemCols > 128 ? sm_count * 9 / 10 : sm_count * 27 / 20;
+  p.cluster = std::max(1, std::min({kMaxCluster, num_kb, ctas / std::max(1, tiles)}));
+  if (p.cluster == 1 && L::kOwnSlots && num_kb >= 4 && tiles > sm_count && tiles <= ctas) p.cluster = 2;
   auto x_area = [&] {  // this CTA's slice of A, quantised
     return FUSED ? ceil_div(num_kb, p.cluster) * (L::kX + L::kT * L::kXSTile) + kFp4TileBytes : 0u;
   };
@@ -440,7 +457,9 @@ RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   const int local = ceil_div(num_kb, p.cluster);
   const uint32_t x_bytes = x_area();
   const uint32_t slots = p.cluster > 1 ? L::slots(p.cluster) : 0;
-  const uint32_t budget = per_sm == 2 ? 108 * 1024 : 218 * 1024;
+  // Shared memory for the ring: a third of an SM for narrow tiles that split K (this launch's CTAs and the next's
+  // are resident together), half of one otherwise, all of it for 512 TMEM columns.
+  const uint32_t budget = (L::kTmemCols > 256 ? 218 : L::kOwnSlots && p.cluster > 1 ? 72 : 108) * 1024;
   const uint32_t fixed = x_bytes + (L::kOwnSlots ? slots : 0);
   p.ring = fixed + 2 * L::kStage > budget ? 2 : static_cast<int>((budget - fixed) / L::kStage);
   p.ring = std::max(2, std::min({kMaxRing, local, p.ring}));
@@ -547,8 +566,13 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
 }
 
 // Whether w4a4_linear quantises x inside the product: up to 16 rows, of a length whose slice fits beside the ring (an
-// eighth of 32768 columns: 16 stages of at most 3 KB).
-bool fp4_fused_ok(int M, int K) { return M <= 16 && K <= 32768; }
+// eighth of 32768 columns: 16 stages of at most 3 KB), and where every 128 weight rows quantising x anew costs
+// less than a launch for it: measured at M K tiles = 3.1 million 8.0 against 8.5 us (16 rows 4096->6144) and
+// 13.1 against 13.4 (4 rows 4096->24576), at 6.3 million 14.9 against 13.7 (8 rows 4096->24576) and 12.5 against
+// 11.4 (16 rows 12288->4096).
+bool fp4_fused_ok(int M, int N, int K) {
+  return M <= 16 && K <= 32768 && static_cast<int64_t>(M) * K * ceil_div(N, kTileN) <= (1 << 22);
+}
 
 int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
                     const void* w_scales, void* y, int64_t y_ld, int M, int N, int K, int format, float alpha,

@@ -18,7 +18,7 @@ int fp4_matmul_pair(const void* a_codes, int64_t a_ld, const void* a_scales, con
                     const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
                     cudaStream_t stream);
 
-bool fp4_fused_ok(int M, int K);
+bool fp4_fused_ok(int M, int N, int K);
 int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
                     const void* w_scales, void* y, int64_t y_ld, int M, int N, int K, int format, float alpha,
                     cudaStream_t stream);
@@ -61,7 +61,7 @@ extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t
   if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   size_t offset;
   *bytes = 0;
-  if (!fp4_fused_ok(M, K)) workspace_layout(M, K, format, &offset, bytes);
+  if (!fp4_fused_ok(M, N, K)) workspace_layout(M, K, format, &offset, bytes);
   return ASHQK_OK;
 }
 
@@ -74,7 +74,7 @@ extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gat
   if (!fp4_global_scale_ok(format, x_scale) || !fp4_global_scale_ok(format, w_scale)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(w_codes, w_ld, w_scales, K)) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (fp4_fused_ok(M, K))
+  if (fp4_fused_ok(M, N, K))
     return fp4_linear_rows(x, x_ld, dtype, gated != 0, x_scale, w_codes, w_ld, w_scales, y, y_ld, M, N, K, format,
                            x_scale * w_scale, st);
   size_t offset, bytes;
