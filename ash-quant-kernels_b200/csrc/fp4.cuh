@@ -79,28 +79,69 @@ __device__ __forceinline__ uint32_t fp4_scale_of(uint32_t amax, const Fp4Quant& 
   }
 }
 
-// A value over its scale, before rounding to E2M1. For NVFP4 the rounded quotient and not the product with the
-// reciprocal, which would move exact ties (x = 0.75 d, which 16-bit inputs meet often) off the border.
-template <int FMT>
-__device__ __forceinline__ float fp4_scaled(float v, float d, float r) {
-  return FMT == ASHQK_MXFP4 ? v * r : quotient(v, d, r);
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
 }
 
-// Eight scaled values -> eight E2M1 codes, the first in the lowest four bits; to nearest even, held
-// to +-6.
-__device__ __forceinline__ uint32_t fp4_pack8(const float (&v)[8]) {
+// Four pairs of scaled values -> eight E2M1 codes, the first in the lowest four bits; to nearest even, held to +-6.
+__device__ __forceinline__ uint32_t fp4_pack8(const uint64_t* v) {
   uint32_t r;
   asm("{\n"
       " .reg .b8 b0, b1, b2, b3;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n"
-      " cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      " .reg .f32 l, h;\n"
+      " mov.b64 {l, h}, %1;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b0, h, l;\n"
+      " mov.b64 {l, h}, %2;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b1, h, l;\n"
+      " mov.b64 {l, h}, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b2, h, l;\n"
+      " mov.b64 {l, h}, %4;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 b3, h, l;\n"
       " mov.b32 %0, {b0, b1, b2, b3};\n"
       "}\n"
       : "=r"(r)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+      : "l"(v[0]), "l"(v[1]), "l"(v[2]), "l"(v[3]));
   return r;
+}
+
+// Sixteen values of one block (NVFP4) or of half a block whose other half the neighbouring lane has (MXFP4) -> their
+// codes and the block's scale byte. `amax`: the largest magnitude of these sixteen, as fp32 bits. All lanes of
+// the warp call it together.
+//
+// For NVFP4 a code is the rounded quotient's, by quotient()'s arithmetic in pairs, and not that of the product with
+// the reciprocal, which would move exact ties (x = 0.75 d, which 16-bit inputs meet often) off the border.
+template <int FMT>
+__device__ __forceinline__ uint32_t fp4_quantize16(float (&v)[16], uint32_t amax, const Fp4Quant& q, uint2* codes) {
+  if (FMT == ASHQK_MXFP4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  float d, r;
+  const uint32_t byte = fp4_scale_of<FMT>(amax, q, &d, &r);
+  if (FMT == ASHQK_NVFP4 && byte == 126u) {  // perhaps beyond the largest scale: quotients without bound
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = fminf(fmaxf(v[i], -8.0f * d), 8.0f * d);
+  }
+  const uint64_t r2 = f32x2(r, r), nd2 = f32x2(-d, -d);
+  uint64_t s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint64_t x = f32x2(v[2 * i], v[2 * i + 1]);
+    s[i] = mul2(x, r2);
+    if (FMT == ASHQK_NVFP4) s[i] = fma2(fma2(s[i], nd2, x), r2, s[i]);
+  }
+  *codes = make_uint2(fp4_pack8(s), fp4_pack8(s + 4));
+  return byte;
 }
 
 // Eight E2M1 codes -> values.
@@ -192,63 +233,83 @@ __device__ __forceinline__ uint4 ld_once_v4(const void* p) {
   return v;
 }
 
-// Eight consecutive 16-bit values as they lie in memory: `vec` when p is 16-byte aligned and all eight exist, else
-// one by one with zeros from `count` on.
+// Sixteen consecutive values as they lie in memory. `align`: what the caller knows of every chunk's address, 32 or 16
+// bytes, else 0 (or a chunk that ends early): then one by one, with zeros from `count` on.
 template <typename T>
-__device__ __forceinline__ uint4 load8_raw(const T* p, int count, bool vec) {
-  static_assert(sizeof(T) == 2, "16-bit types");
-  if (vec) return ld_once_v4(p);
-  uint32_t w[4];
+struct Raw16 {
+  uint32_t w[4 * sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, int count, int align, Raw16<T>& r) {
+  if (align == 32) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p) + 2 * i;
-    w[i] = (2 * i < count ? h[0] : 0u) | ((2 * i + 1 < count ? h[1] : 0u) << 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-  unpack2<T>(u.x, v[0], v[1]);
-  unpack2<T>(u.y, v[2], v[3]);
-  unpack2<T>(u.z, v[4], v[5]);
-  unpack2<T>(u.w, v[6], v[7]);
-}
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int count, bool vec, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    unpack8<T>(load8_raw(p, count, vec), v);
-  } else if (vec) {
-    const uint4 a = ld_once_v4(p), b = ld_once_v4(p + 4);
-    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+      asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(r.w[8 * i]), "=r"(r.w[8 * i + 1]), "=r"(r.w[8 * i + 2]), "=r"(r.w[8 * i + 3]), "=r"(r.w[8 * i + 4]),
+                     "=r"(r.w[8 * i + 5]), "=r"(r.w[8 * i + 6]), "=r"(r.w[8 * i + 7])
+                   : "l"(reinterpret_cast<const uint32_t*>(p) + 8 * i)
+                   : "memory");
+  } else if (align == 16) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) {
+      const uint4 u = ld_once_v4(reinterpret_cast<const uint4*>(p) + i);
+      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
+    }
+  } else if constexpr (sizeof(T) == 2) {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      r.w[i] = (2 * i < count ? h[2 * i] : 0u) | ((2 * i + 1 < count ? h[2 * i + 1] : 0u) << 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < count ? p[i] : 0.0f;
+    for (int i = 0; i < 16; ++i) r.w[i] = i < count ? __float_as_uint(p[i]) : 0u;
+  }
+}
+// What is known of p + 16 j elements for every row of a matrix.
+inline int chunk_align(const void* p, int64_t ld, int size) {
+  return aligned(p, 32) && ld * size % 32 == 0 ? 32 : aligned(p, 16) && ld * size % 16 == 0 ? 16 : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const Raw16<T>& r, float (&v)[16]) {
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) unpack2<T>(r.w[i], v[2 * i], v[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r.w[i]);
+  }
+}
+
+// The largest magnitude, as fp32 bits: as an unsigned number those order finite < infinity < NaN.
+__device__ __forceinline__ uint32_t abs_max16(const float (&v)[16]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t abs_max16(const Raw16<T>& r) {
+  if constexpr (sizeof(T) == 2) {  // 16-bit patterns have the same order
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, r.w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      return m << 16;
+    else
+      return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, r.w[i] & 0x7fffffffu);
+    return m;
   }
 }
 
 // silu(gate) * up in fp32. exp overflows to infinity for gates below -88 and the quotient is then 0.
 __device__ __forceinline__ float silu_mul(float gate, float up) {
   return __fdividef(gate, 1.0f + __expf(-gate)) * up;
-}
-
-// The largest magnitude of eight 16-bit values, as the fp32 bit pattern of its absolute value.
-template <typename T>
-__device__ __forceinline__ uint32_t abs_max8_raw(const uint4& u) {
-  uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu), __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu));
-  m = max(m & 0xffffu, m >> 16);
-  if constexpr (std::is_same_v<T, __nv_bfloat16>)
-    return m << 16;
-  else
-    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
-}
-
-// The largest bit pattern of |v|: as an unsigned number it orders finite < infinity < NaN.
-__device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
 }
 
 }  // namespace ashqk

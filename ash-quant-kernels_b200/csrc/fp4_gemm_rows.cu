@@ -48,7 +48,8 @@ struct RowsArgs {
   uint32_t off_x, off_slots, off_bar;  // shared memory after the ring
   float alpha;
   Fp4Quant xq;
-  int bf16, gated, vec;
+  int bf16, gated;
+  int align;  // of 16-column chunks of a 16-bit A
 };
 
 template <int FMT, int NT, bool FUSED>
@@ -95,63 +96,64 @@ __device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
 }
 
-// Quantises columns [256 kb0, 256 kb1) of A's rows into shared memory. Eight columns per thread, a block's
-// lanes adjacent, as in the quantiser proper; two chunks' loads in flight.
+// Quantises columns [256 kb0, 256 kb1) of A's rows into shared memory, sixteen columns per thread, as the quantiser
+// proper does.
 template <int FMT, int NT, typename T, bool GATED>
 __device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int kb1, uint32_t codes, uint32_t scales, int tid) {
   using L = RowsShape<FMT, NT, true>;
-  constexpr int kLanes = fp4_block(FMT) / 8;
-  constexpr int kBatch = 2;
+  constexpr int kLanes = fp4_block(FMT) / 16;
+  constexpr int kBatch = GATED ? 1 : 2;  // chunks whose loads are in flight together
   constexpr int kStep = 32 * kQuantWarps;
-  const int chunks = (kb1 - kb0) * 32;  // of a row: a multiple of 32, so that warps stay in one row
+  const int chunks = (kb1 - kb0) * 16;  // of a row
+  const int total = a.M * chunks;
   const T* x = static_cast<const T*>(a.x);
-  int m = 0, c = tid;  // row and chunk
-  while (c >= chunks) c -= chunks, ++m;
-  while (m < a.M) {
-    uint4 g[kBatch], u[kBatch];
-    int bm[kBatch], bc[kBatch];
+  for (int i0 = tid; (i0 & ~31) < total; i0 += kBatch * kStep) {  // whole warps
+    Raw16<T> g[kBatch], u[GATED ? kBatch : 1];
+    int row[kBatch], chunk[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      bm[b] = m, bc[b] = c;
-      g[b] = u[b] = make_uint4(0, 0, 0, 0);
-      const int k0 = kb0 * kFp4BlockK + c * 8;
-      if (m < a.M && k0 < a.K) {
-        const T* p = x + m * a.x_ld + k0;
-        const bool whole = a.vec && k0 + 8 <= a.K;
-        g[b] = load8_raw(p, a.K - k0, whole);
-        if (GATED) u[b] = load8_raw(p + a.K, a.K - k0, whole);
+      const int i = i0 + b * kStep;
+      row[b] = i / chunks;
+      chunk[b] = i - row[b] * chunks;
+      const int k0 = kb0 * kFp4BlockK + chunk[b] * 16;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[b].w[j] = 0;
+        if (GATED) u[b].w[j] = 0;
       }
-      c += kStep;
-      while (c >= chunks) c -= chunks, ++m;
+      if (i < total && k0 < a.K) {
+        const T* p = x + row[b] * a.x_ld + k0;
+        const int align = k0 + 16 <= a.K ? a.align : 0;
+        load16<T>(p, a.K - k0, align, g[b]);
+        if (GATED) load16<T>(p + a.K, a.K - k0, align, u[b]);
+      }
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      if (bm[b] >= a.M) break;  // whole warps
-      float v[8];
-      unpack8<T>(g[b], v);
+      if (((i0 + b * kStep) & ~31) >= total) break;  // whole warps
+      float v[16];
+      unpack16<T>(g[b], v);
       uint32_t amax;
-      if (GATED) {
-        float w[8];
-        unpack8<T>(u[b], w);
+      if constexpr (GATED) {
+        float w[16];
+        unpack16<T>(u[b], w);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], w[j]);
-        amax = abs_max8(v);
+        for (int j = 0; j < 16; ++j) v[j] = silu_mul(v[j], w[j]);
+        amax = abs_max16(v);
       } else {
-        amax = abs_max8_raw<T>(g[b]);
+        amax = abs_max16(g[b]);
       }
-#pragma unroll
-      for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-      float d, r;
-      const uint32_t byte = fp4_scale_of<FMT>(amax, a.xq, &d, &r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], d, r);
-      const int row = bm[b], kb = bc[b] >> 5, cc = bc[b] & 31;
-      const uint32_t at = codes + kb * L::kX + (row >> 3) * 1024 + (row & 7) * 128 + (((cc >> 2) ^ (row & 7)) << 4) + (cc & 3) * 4;
-      asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(fp4_pack8(v)) : "memory");
-      if (cc % kLanes == 0) {
-        const int block = cc / kLanes;
-        const uint32_t s = scales + (kb * L::kT + (block >> 2)) * L::kXSTile + row * 16 + (block & 3);
-        asm volatile("st.shared.u8 [%0], %1;" ::"r"(s), "r"(byte) : "memory");
+      uint2 c;
+      const uint32_t byte = fp4_quantize16<FMT>(v, amax, a.xq, &c);
+      if (i0 + b * kStep < total) {
+        const int m = row[b], kb = chunk[b] >> 4, cc = chunk[b] & 15;
+        const uint32_t at = codes + kb * L::kX + (m >> 3) * 1024 + (m & 7) * 128 + (((cc >> 1) ^ (m & 7)) << 4) + (cc & 1) * 8;
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c.x), "r"(c.y) : "memory");
+        if (cc % kLanes == 0) {
+          const int block = cc / kLanes;
+          const uint32_t s = scales + (kb * L::kT + (block >> 2)) * L::kXSTile + m * 16 + (block & 3);
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"(s), "r"(byte) : "memory");
+        }
       }
     }
   }
@@ -586,7 +588,7 @@ int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_
   a.x_ld = x_ld;
   a.xq = fp4_quant_params(x_gs);
   a.gated = gated;
-  a.vec = aligned(x, 16) && x_ld % 8 == 0 && (!gated || K % 8 == 0);
+  a.align = std::min(chunk_align(x, x_ld, 2), gated ? chunk_align(nullptr, K, 2) : 32);
   const int nt = M <= 8 ? 8 : 16;
   return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, true, stream)
                                : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, true, stream);

@@ -1,10 +1,11 @@
 // Quantising rows to microscaled 4-bit floating point, plain or of silu(gate) * up, and reading
 // them back.
 //
-// One thread takes chunks of eight columns (16 bytes of a 16-bit input, 4 bytes of codes); the lanes of a block
-// (4 for MXFP4, 2 for NVFP4) share its largest magnitude by shuffles, so every value is read once and
-// nothing passes through shared memory. HBM-bound: a value costs its input, half a byte of code and
-// 1/32 or 1/16 byte of scale. Where there are enough chunks a thread takes four, their loads in flight together.
+// One thread takes chunks of sixteen columns (one 32-byte load of a 16-bit input, 8 bytes of codes): an NVFP4 block, or
+// half an MXFP4 block, whose two lanes share its largest magnitude by a shuffle. Every value is read once and
+// nothing passes through shared memory. A value costs its input, half a byte of code and 1/32 or 1/16
+// byte of scale; the arithmetic is in pairs (f32x2) because at HBM speed an SM has some eleven instruction slots
+// per value. Where there are enough chunks a thread takes two, their loads in flight together.
 #include <algorithm>
 
 #include "fp4.cuh"
@@ -35,78 +36,64 @@ template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
 __global__ void __launch_bounds__(kQuantThreads)
     quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, int64_t codes_ld,
                         uint8_t* __restrict__ scales, int64_t row0, uint32_t total, int K, FastDiv by_chunks, Fp4Quant q,
-                        bool vec, int early) {
-  constexpr int kLanes = fp4_block(FMT) / 8;  // lanes of a block
+                        int align, int early) {
+  constexpr int kLanes = fp4_block(FMT) / 16;  // lanes of a block
   pdl_wait();
   if (early) pdl_launch_dependents();
-  const uint32_t chunks = by_chunks.d;  // of a row; a multiple of 4: a block's lanes share a row
+  const uint32_t chunks = by_chunks.d;  // of a row; an even number: a block's lanes share a row
   const int64_t tiles = fp4_scale_tiles(K, FMT);
   const uint32_t first = blockIdx.x * (kQuantThreads * BATCH) + threadIdx.x;
-  uint4 g[BATCH], u[BATCH];
-  float gf[sizeof(T) == 4 ? BATCH : 1][8], uf[sizeof(T) == 4 ? BATCH : 1][8];
+  Raw16<T> g[BATCH], u[GATED ? BATCH : 1];
+  uint32_t row[BATCH], chunk[BATCH];
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) {
     const uint32_t i = first + b * kQuantThreads;
-    const uint32_t r = divide(i, by_chunks);
-    const int k0 = static_cast<int>(i - r * chunks) * 8;
-    const bool live = i < total && k0 < K;
-    const T* p = x + (row0 + r) * x_ld + k0;
-    const bool whole = vec && k0 + 8 <= K;
-    if constexpr (sizeof(T) == 2) {
-      g[b] = u[b] = make_uint4(0, 0, 0, 0);
-      if (live) g[b] = load8_raw(p, K - k0, whole);
-      if (live && GATED) u[b] = load8_raw(p + K, K - k0, whole);
-    } else {
+    row[b] = divide(i, by_chunks);
+    chunk[b] = i - row[b] * chunks;
+    const int k0 = static_cast<int>(chunk[b]) * 16;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) gf[b][j] = uf[b][j] = 0.0f;
-      if (live) load8<T>(p, K - k0, whole, gf[b]);
-      if (live && GATED) load8<T>(p + K, K - k0, whole, uf[b]);
+    for (int j = 0; j < static_cast<int>(4 * sizeof(T)); ++j) {
+      g[b].w[j] = 0;
+      if (GATED) u[b].w[j] = 0;
+    }
+    if (i < total && k0 < K) {
+      const T* p = x + (row0 + row[b]) * x_ld + k0;
+      const int al = k0 + 16 <= K ? align : 0;
+      load16<T>(p, K - k0, al, g[b]);
+      if (GATED) load16<T>(p + K, K - k0, al, u[b]);
     }
   }
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) {
-    const uint32_t i = first + b * kQuantThreads;
-    float v[8], w[8];
+    float v[16];
+    unpack16<T>(g[b], v);
     uint32_t amax;
-    if constexpr (sizeof(T) == 2) {
-      unpack8<T>(g[b], v);
-      if (GATED) unpack8<T>(u[b], w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = gf[b][j], w[j] = uf[b][j];
-    }
     if constexpr (GATED) {
+      float w[16];
+      unpack16<T>(u[b], w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], w[j]);
-      amax = abs_max8(v);
-    } else if constexpr (sizeof(T) == 2) {
-      amax = abs_max8_raw<T>(g[b]);
+      for (int j = 0; j < 16; ++j) v[j] = silu_mul(v[j], w[j]);
+      amax = abs_max16(v);
     } else {
-      amax = abs_max8(v);
+      amax = abs_max16(g[b]);
     }
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    float d, r;
-    uint32_t bytes = fp4_scale_of<FMT>(amax, q, &d, &r);
-    const uint32_t rr = divide(i, by_chunks);
-    const uint32_t chunk = i - rr * chunks;
-    const int64_t row = row0 + rr;
-    const int block = static_cast<int>(chunk / kLanes);
+    uint2 c;
+    uint32_t bytes = fp4_quantize16<FMT>(v, amax, q, &c);
+    const int block = static_cast<int>(chunk[b] / kLanes);
     if (WHOLE) {
       bytes <<= 8 * (block & 3);
       bytes |= __shfl_xor_sync(0xffffffffu, bytes, kLanes);
       bytes |= __shfl_xor_sync(0xffffffffu, bytes, 2 * kLanes);
     }
-    if (i >= total) continue;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = fp4_scaled<FMT>(v[j], d, r);
-    *reinterpret_cast<uint32_t*>(codes + row * codes_ld + chunk * 4) = fp4_pack8(v);
-    uint8_t* s = scales + fp4_scale_offset(row, block, tiles);
+    if (first + b * kQuantThreads >= total) continue;
+    const int64_t r = row0 + row[b];
+    *reinterpret_cast<uint2*>(codes + r * codes_ld + chunk[b] * 8) = c;
+    uint8_t* s = scales + fp4_scale_offset(r, block, tiles);
     if (WHOLE) {
-      if (chunk % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
-    } else if (chunk % kLanes == 0) {
+      if (chunk[b] % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
+    } else if (chunk[b] % kLanes == 0) {
       *s = static_cast<uint8_t>(bytes);
-      if (chunk + kLanes == chunks)  // the tile's padding blocks
+      if (chunk[b] + kLanes == chunks)  // the tile's padding blocks
         for (int k = block + 1; k & 3; ++k) *++s = 0;
     }
   }
@@ -175,14 +162,14 @@ int launch_pdl(void (*kernel)(Params...), int64_t blocks, int threads, cudaStrea
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) == cudaSuccess ? ASHQK_OK : ASHQK_ERR_CUDA;
 }
 
-constexpr int kBatch = 4;
-// From here on four chunks per thread still leave every SM two blocks (148 SMs).
-constexpr int64_t kBatchChunks = 2 * 148 * kQuantThreads * kBatch;
+constexpr int kQuantBatch = 2, kDequantBatch = 4;
+// Whether `batch` chunks per thread still leave every SM two blocks (148 SMs).
+constexpr bool many_chunks(int64_t chunks, int batch) { return chunks >= 2 * 148 * kQuantThreads * batch; }
 
 // Calls launch(row0, chunks, blocks of kQuantThreads * batch) for slabs of rows with fewer than 2^31 chunks.
 template <typename F>
 int for_slabs(int64_t rows, int64_t chunks, int batch, F launch) {
-  const int64_t most = std::max<int64_t>(1, ((1ll << 31) - 2 * kQuantThreads * kBatch) / chunks);
+  const int64_t most = std::max<int64_t>(1, ((1ll << 31) - 8 * kQuantThreads) / chunks);
   for (int64_t row0 = 0; row0 < rows; row0 += most) {
     const int64_t total = std::min(most, rows - row0) * chunks;
     if (const int rc = launch(row0, static_cast<uint32_t>(total), ceil_div64(total, kQuantThreads * batch))) return rc;
@@ -193,12 +180,13 @@ int for_slabs(int64_t rows, int64_t chunks, int batch, F launch) {
 template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
 int quantize_launch(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
                     bool early, cudaStream_t stream) {
-  const bool vec = aligned(x, 16) && (x_ld * sizeof(T)) % 16 == 0 && (!GATED || (K * sizeof(T)) % 16 == 0);
-  const int64_t chunks = fp4_padded_k(K) / 8;
+  int align = chunk_align(x, x_ld, sizeof(T));
+  if (GATED) align = std::min(align, chunk_align(nullptr, K, sizeof(T)));
+  const int64_t chunks = fp4_padded_k(K) / 16;
   return for_slabs(M, chunks, BATCH, [&](int64_t row0, uint32_t total, int64_t blocks) {
     return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, BATCH, WHOLE>, blocks, kQuantThreads, stream,
                       static_cast<const T*>(x), x_ld, codes, codes_ld, scales, row0, total, K,
-                      fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(gs), vec, early);
+                      fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(gs), align, early);
   });
 }
 
@@ -207,9 +195,9 @@ int quantize_shaped(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_l
                     bool early, cudaStream_t stream) {
   const int64_t kp = fp4_padded_k(K);
   const bool whole = kp % (4 * fp4_block(FMT)) == 0;
-  const bool many = M * (kp / 8) >= kBatchChunks;
-  return (whole ? many ? quantize_launch<FMT, T, GATED, kBatch, true> : quantize_launch<FMT, T, GATED, 1, true>
-          : many ? quantize_launch<FMT, T, GATED, kBatch, false>
+  const bool many = many_chunks(M * (kp / 16), kQuantBatch);
+  return (whole ? many ? quantize_launch<FMT, T, GATED, kQuantBatch, true> : quantize_launch<FMT, T, GATED, 1, true>
+          : many ? quantize_launch<FMT, T, GATED, kQuantBatch, false>
                  : quantize_launch<FMT, T, GATED, 1, false>)(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
 }
 
@@ -225,9 +213,9 @@ int dequantize_typed(const uint8_t* codes, int64_t codes_ld, const uint8_t* scal
                      int K, float gs, cudaStream_t stream) {
   const bool vec = aligned(out, 16) && (out_ld * sizeof(T)) % 16 == 0;
   const int64_t chunks = (K + 7) / 8;
-  const bool many = M * chunks >= kBatchChunks;
-  return for_slabs(M, chunks, many ? kBatch : 1, [&](int64_t row0, uint32_t total, int64_t blocks) {
-    return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kBatch> : dequantize_fp4_kernel<FMT, T, 1>, blocks,
+  const bool many = many_chunks(M * chunks, kDequantBatch);
+  return for_slabs(M, chunks, many ? kDequantBatch : 1, [&](int64_t row0, uint32_t total, int64_t blocks) {
+    return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kDequantBatch> : dequantize_fp4_kernel<FMT, T, 1>, blocks,
                       kQuantThreads, stream, codes, codes_ld, scales, static_cast<T*>(out), out_ld, row0, total, K,
                       fast_div(static_cast<uint32_t>(chunks)), gs, vec);
   });
