@@ -45,13 +45,20 @@ inline Fp4Quant fp4_quant_params(float gs) {
   return {gs, six, 1.0f / six};
 }
 
-// v / d, rounded to fp32 as one division is, from r = 1 / d correctly rounded: the product v r is off by at most a
-// unit in the last place, and one step with the exact residual corrects it (P. W. Markstein, Computation of
-// elementary functions on the IBM RISC System/6000 processor, IBM J. Res. Dev. 34, 1990). Quotients are cut
-// off at +-1024, beyond what either format holds, so that the residual stays finite.
+// v / d from an r near 1 / d (within two units in the last place): the product v r, corrected once by the exact
+// residual, differs from the quotient rounded once only where that lies within 2^-20 units of halfway between two
+// fp32 values -- never where the quotient is an fp32 value, as the borders between codes are (after
+// P. W. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, IBM J. Res.
+// Dev. 34, 1990). Quotients are cut off at +-1024, beyond what either format holds, so that the residual
+// stays finite.
 __device__ __forceinline__ float quotient(float v, float d, float r) {
   const float q = fminf(fmaxf(v * r, -1024.0f), 1024.0f);
   return fmaf(fmaf(-q, d, v), r, q);
+}
+__device__ __forceinline__ float reciprocal_approx(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
 }
 
 // The scale of a block whose largest magnitude has the fp32 bit pattern `amax` (sign cleared): its byte, its value d
@@ -74,7 +81,7 @@ __device__ __forceinline__ uint32_t fp4_scale_of(uint32_t amax, const Fp4Quant& 
     uint32_t h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(byte)));
     *d = __low2float(u32_as_h2(h2)) * q.gs;
-    *r = *d > 0.0f ? __frcp_rn(*d) : 0.0f;
+    *r = *d > 0.0f ? reciprocal_approx(*d) : 0.0f;
     return byte;
   }
 }
@@ -117,17 +124,12 @@ __device__ __forceinline__ uint32_t fp4_pack8(const uint64_t* v) {
   return r;
 }
 
-// Sixteen values of one block (NVFP4) or of half a block whose other half the neighbouring lane has (MXFP4) -> their
-// codes and the block's scale byte. `amax`: the largest magnitude of these sixteen, as fp32 bits. All lanes of
-// the warp call it together.
+// The codes of sixteen values that share the scale fp4_scale_of gave.
 //
-// For NVFP4 a code is the rounded quotient's, by quotient()'s arithmetic in pairs, and not that of the product with
+// For NVFP4 a code is the corrected quotient's, by quotient()'s arithmetic in pairs, and not that of the product with
 // the reciprocal, which would move exact ties (x = 0.75 d, which 16-bit inputs meet often) off the border.
 template <int FMT>
-__device__ __forceinline__ uint32_t fp4_quantize16(float (&v)[16], uint32_t amax, const Fp4Quant& q, uint2* codes) {
-  if (FMT == ASHQK_MXFP4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  float d, r;
-  const uint32_t byte = fp4_scale_of<FMT>(amax, q, &d, &r);
+__device__ __forceinline__ uint2 fp4_codes16(float* v, uint32_t byte, float d, float r) {
   if (FMT == ASHQK_NVFP4 && byte == 126u) {  // perhaps beyond the largest scale: quotients without bound
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = fminf(fmaxf(v[i], -8.0f * d), 8.0f * d);
@@ -140,12 +142,23 @@ __device__ __forceinline__ uint32_t fp4_quantize16(float (&v)[16], uint32_t amax
     s[i] = mul2(x, r2);
     if (FMT == ASHQK_NVFP4) s[i] = fma2(fma2(s[i], nd2, x), r2, s[i]);
   }
-  *codes = make_uint2(fp4_pack8(s), fp4_pack8(s + 4));
+  return make_uint2(fp4_pack8(s), fp4_pack8(s + 4));
+}
+
+// Sixteen values of one block (NVFP4) or of half a block whose other half the neighbouring lane has (MXFP4) -> their
+// codes and the block's scale byte. `amax`: the largest magnitude of these sixteen, as fp32 bits. All lanes of
+// the warp call it together.
+template <int FMT>
+__device__ __forceinline__ uint32_t fp4_quantize16(float (&v)[16], uint32_t amax, const Fp4Quant& q, uint2* codes) {
+  if (FMT == ASHQK_MXFP4) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  float d, r;
+  const uint32_t byte = fp4_scale_of<FMT>(amax, q, &d, &r);
+  *codes = fp4_codes16<FMT>(v, byte, d, r);
   return byte;
 }
 
 // Eight E2M1 codes -> values.
-__device__ __forceinline__ void fp4_unpack8(uint32_t codes, float (&v)[8]) {
+__device__ __forceinline__ void fp4_unpack8(uint32_t codes, float* v) {
   uint32_t h[4];
   asm("{\n"
       " .reg .b8 b0, b1, b2, b3;\n"
@@ -233,45 +246,63 @@ __device__ __forceinline__ uint4 ld_once_v4(const void* p) {
   return v;
 }
 
-// Sixteen consecutive values as they lie in memory. `align`: what the caller knows of every chunk's address, 32 or 16
-// bytes, else 0 (or a chunk that ends early): then one by one, with zeros from `count` on.
+// Sixteen consecutive values as they lie in memory. `align`: what the caller knows of the address, 32 or 16 bytes, and
+// then all sixteen exist; else 0, and of the values those from `count` on read as zero. Without alignment the
+// 16-byte granules that hold the values are loaded whole (a granule with a byte of an allocation is in it) and
+// shifted into place.
 template <typename T>
 struct Raw16 {
   uint32_t w[4 * sizeof(T)];
 };
 template <typename T>
 __device__ __forceinline__ void load16(const T* p, int count, int align, Raw16<T>& r) {
+  constexpr int kWords = 4 * sizeof(T);
   if (align == 32) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    for (int i = 0; i < kWords; i += 8)
       asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(r.w[8 * i]), "=r"(r.w[8 * i + 1]), "=r"(r.w[8 * i + 2]), "=r"(r.w[8 * i + 3]), "=r"(r.w[8 * i + 4]),
-                     "=r"(r.w[8 * i + 5]), "=r"(r.w[8 * i + 6]), "=r"(r.w[8 * i + 7])
-                   : "l"(reinterpret_cast<const uint32_t*>(p) + 8 * i)
+                   : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]),
+                     "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
+                   : "l"(reinterpret_cast<const uint32_t*>(p) + i)
                    : "memory");
   } else if (align == 16) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)); ++i) {
-      const uint4 u = ld_once_v4(reinterpret_cast<const uint4*>(p) + i);
-      r.w[4 * i] = u.x, r.w[4 * i + 1] = u.y, r.w[4 * i + 2] = u.z, r.w[4 * i + 3] = u.w;
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 u = ld_once_v4(reinterpret_cast<const uint32_t*>(p) + i);
+      r.w[i] = u.x, r.w[i + 1] = u.y, r.w[i + 2] = u.z, r.w[i + 3] = u.w;
     }
-  } else if constexpr (sizeof(T) == 2) {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      r.w[i] = (2 * i < count ? h[2 * i] : 0u) | ((2 * i + 1 < count ? h[2 * i + 1] : 0u) << 16);
   } else {
+    const uintptr_t first = reinterpret_cast<uintptr_t>(p), last = first + sizeof(T) * min(count, 16);
+    const uint32_t off = first & 15u;
+    uint32_t w[kWords + 4];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r.w[i] = i < count ? __float_as_uint(p[i]) : 0u;
+    for (int i = 0; i < kWords + 4; i += 4) {
+      const uintptr_t at = first - off + 4 * i;
+      const uint4 u = at < last ? ld_once_v4(reinterpret_cast<const void*>(at)) : make_uint4(0, 0, 0, 0);
+      w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+    }
+#pragma unroll
+    for (int i = 0; i < kWords + 3; ++i) w[i] = off & 4u ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) w[i] = off & 8u ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        r.w[i] = off & 2u ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+        if (2 * i + 1 >= count) r.w[i] = 2 * i < count ? r.w[i] & 0xffffu : 0u;
+      } else {
+        r.w[i] = i < count ? w[i] : 0u;
+      }
+    }
   }
 }
-// What is known of p + 16 j elements for every row of a matrix.
+// What is known of the address of column 16 j for every row of a matrix.
 inline int chunk_align(const void* p, int64_t ld, int size) {
   return aligned(p, 32) && ld * size % 32 == 0 ? 32 : aligned(p, 16) && ld * size % 16 == 0 ? 16 : 0;
 }
 
 template <typename T>
-__device__ __forceinline__ void unpack16(const Raw16<T>& r, float (&v)[16]) {
+__device__ __forceinline__ void unpack16(const Raw16<T>& r, float* v) {
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) unpack2<T>(r.w[i], v[2 * i], v[2 * i + 1]);
@@ -282,7 +313,7 @@ __device__ __forceinline__ void unpack16(const Raw16<T>& r, float (&v)[16]) {
 }
 
 // The largest magnitude, as fp32 bits: as an unsigned number those order finite < infinity < NaN.
-__device__ __forceinline__ uint32_t abs_max16(const float (&v)[16]) {
+__device__ __forceinline__ uint32_t abs_max16(const float* v) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);

@@ -83,6 +83,12 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ uint16_t lds_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+
 // 64 fp32 columns of one row, times alpha, as 16-bit pairs.
 template <typename T>
 __device__ __forceinline__ void round_row64(const uint32_t (&r0)[32], const uint32_t (&r1)[32], float alpha, uint32_t (&h)[32]) {
@@ -272,25 +278,31 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_pair_kernel(const __grid_cons
         else
           round_row64<__half>(r0, r1, a.alpha, v);
         const int n = tn * kBN + col;
-        if (a.tma_y) {
-          // Through shared memory in the swizzled layout (conflict-free: eight lanes write eight 16-byte columns) and
-          // out as one box of whole 128-byte rows.
-          if (lane == 0) bulk_wait_read();
-          __syncwarp();
+        // Through shared memory in the swizzled layout (conflict-free: eight lanes write eight 16-byte columns).
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            sts_v4(out + lane * 128 + ((c ^ (lane & 7)) << 4), make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
+        for (int c = 0; c < 8; ++c)
+          sts_v4(out + lane * 128 + ((c ^ (lane & 7)) << 4), make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]));
+        if (a.tma_y) {  // out as one box of whole 128-byte rows
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < a.M && n < a.N) {
             tma_store_2d(&maps.y, n, row0, smem + L::off_out + (warp - kFirstEpiWarp) * L::kOut);
             bulk_commit();
           }
-        } else if (row0 + lane < a.M) {
-          uint16_t* y = static_cast<uint16_t*>(a.y) + (row0 + lane) * a.y_ld + n;
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (n + i < a.N) y[i] = static_cast<uint16_t>(v[i / 2] >> (16 * (i & 1)));
+        } else {  // rows of any alignment: the warp writes one after the other
+          __syncwarp();
+          uint16_t* y = static_cast<uint16_t*>(a.y) + row0 * a.y_ld + n + lane;
+          const int rows = min(32, a.M - row0);
+          const bool in0 = n + lane < a.N, in1 = n + 32 + lane < a.N;
+#pragma unroll 4
+          for (int i = 0; i < rows; ++i, y += a.y_ld) {
+            const uint32_t at = out + i * 128 + (lane & 7) * 2;
+            if (in0) y[0] = lds_u16(at + (((lane >> 3) ^ (i & 7)) << 4));
+            if (in1) y[32] = lds_u16(at + (((4 + (lane >> 3)) ^ (i & 7)) << 4));
+          }
+          __syncwarp();
         }
       }
       // The other half is only overwritten after the next tile's shared half was handed back, by these warps.

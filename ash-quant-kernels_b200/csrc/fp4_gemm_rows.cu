@@ -569,11 +569,11 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
 
 // Whether w4a4_linear quantises x inside the product: up to 16 rows, of a length whose slice fits beside the ring (an
 // eighth of 32768 columns: 16 stages of at most 3 KB), and where every 128 weight rows quantising x anew costs
-// less than a launch for it: measured at M K tiles = 3.1 million 8.0 against 8.5 us (16 rows 4096->6144) and
-// 13.1 against 13.4 (4 rows 4096->24576), at 6.3 million 14.9 against 13.7 (8 rows 4096->24576) and 12.5 against
-// 11.4 (16 rows 12288->4096).
+// less than a launch for it. Measured (MXFP4, fused against two launches, in a graph): at M K tiles = 6.3 million
+// 12.8 against 15.9 us (8 rows 4096->24576) and 11.2 against 11.7 (16 rows 12288->4096), at 12.6 million 15.3
+// against 16.1 (16 rows 4096->24576; NVFP4 17.2 against 17.2).
 bool fp4_fused_ok(int M, int N, int K) {
-  return M <= 16 && K <= 32768 && static_cast<int64_t>(M) * K * ceil_div(N, kTileN) <= (1 << 22);
+  return M <= 16 && K <= 32768 && static_cast<int64_t>(M) * K * ceil_div(N, kTileN) <= (1 << 24);
 }
 
 int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,

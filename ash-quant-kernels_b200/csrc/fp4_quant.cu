@@ -1,11 +1,10 @@
 // Quantising rows to microscaled 4-bit floating point, plain or of silu(gate) * up, and reading
 // them back.
 //
-// One thread takes chunks of sixteen columns (one 32-byte load of a 16-bit input, 8 bytes of codes): an NVFP4 block, or
-// half an MXFP4 block, whose two lanes share its largest magnitude by a shuffle. Every value is read once and
-// nothing passes through shared memory. A value costs its input, half a byte of code and 1/32 or 1/16
-// byte of scale; the arithmetic is in pairs (f32x2) because at HBM speed an SM has some eleven instruction slots
-// per value. Where there are enough chunks a thread takes two, their loads in flight together.
+// One thread takes 32 columns: two 32-byte loads of a 16-bit input, one 16-byte store of codes, the scales of one MXFP4
+// or two NVFP4 blocks. Every value is read once and nothing passes through shared memory. A value costs its input,
+// half a byte of code and 1/32 or 1/16 byte of scale. At HBM speed an SM has some eleven instruction slots per
+// value, so the arithmetic is in pairs (f32x2) and offsets within a launch are 32-bit.
 #include <algorithm>
 
 #include "fp4.cuh"
@@ -31,118 +30,204 @@ __device__ __forceinline__ uint32_t divide(uint32_t i, const FastDiv& f) {
   return static_cast<uint32_t>((static_cast<uint64_t>(i) * f.mul) >> (31 + f.shift));
 }
 
+constexpr int kChunk = 32;  // columns per thread
+
+// The rows of one launch start at `x`, `codes` and `scales` and lie in fewer than 2^31 bytes of codes.
 // WHOLE: every row is whole tiles of four blocks, whose scales then leave as one 4-byte store.
-template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
-__global__ void __launch_bounds__(kQuantThreads)
-    quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, int64_t codes_ld,
-                        uint8_t* __restrict__ scales, int64_t row0, uint32_t total, int K, FastDiv by_chunks, Fp4Quant q,
+template <int FMT, typename T, bool GATED, bool WHOLE>
+__global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : GATED ? 3 : 4)
+    quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, uint32_t codes_ld,
+                        uint8_t* __restrict__ scales, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks, Fp4Quant q,
                         int align, int early) {
-  constexpr int kLanes = fp4_block(FMT) / 16;  // lanes of a block
+  constexpr int kHalves = kChunk / 16;
+  constexpr int kBlocks = kChunk / fp4_block(FMT);  // of a chunk
   pdl_wait();
   if (early) pdl_launch_dependents();
-  const uint32_t chunks = by_chunks.d;  // of a row; an even number: a block's lanes share a row
-  const int64_t tiles = fp4_scale_tiles(K, FMT);
-  const uint32_t first = blockIdx.x * (kQuantThreads * BATCH) + threadIdx.x;
-  Raw16<T> g[BATCH], u[GATED ? BATCH : 1];
-  uint32_t row[BATCH], chunk[BATCH];
+  const uint32_t i = blockIdx.x * kQuantThreads + threadIdx.x;
+  const uint32_t row = divide(i, by_chunks);
+  const uint32_t chunk = i - row * by_chunks.d;
+  const int k0 = static_cast<int>(chunk) * kChunk;
+  Raw16<T> g[kHalves], u[GATED ? kHalves : 1];
+  const T* p = x + row * x_ld + k0;
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) {
-    const uint32_t i = first + b * kQuantThreads;
-    row[b] = divide(i, by_chunks);
-    chunk[b] = i - row[b] * chunks;
-    const int k0 = static_cast<int>(chunk[b]) * 16;
+  for (int h = 0; h < kHalves; ++h) {
+    const int left = K - k0 - 16 * h;
+    const int al = left >= 16 ? align : 0;
 #pragma unroll
     for (int j = 0; j < static_cast<int>(4 * sizeof(T)); ++j) {
-      g[b].w[j] = 0;
-      if (GATED) u[b].w[j] = 0;
+      g[h].w[j] = 0;
+      if (GATED) u[h].w[j] = 0;
     }
-    if (i < total && k0 < K) {
-      const T* p = x + (row0 + row[b]) * x_ld + k0;
-      const int al = k0 + 16 <= K ? align : 0;
-      load16<T>(p, K - k0, al, g[b]);
-      if (GATED) load16<T>(p + K, K - k0, al, u[b]);
+    if (i < total && left > 0) {
+      load16<T>(p + 16 * h, left, al, g[h]);
+      if (GATED) load16<T>(p + 16 * h + K, left, al, u[h]);
     }
   }
+  float v[kChunk];
+  uint32_t amax[kHalves];
 #pragma unroll
-  for (int b = 0; b < BATCH; ++b) {
-    float v[16];
-    unpack16<T>(g[b], v);
-    uint32_t amax;
+  for (int h = 0; h < kHalves; ++h) {
+    unpack16<T>(g[h], v + 16 * h);
     if constexpr (GATED) {
       float w[16];
-      unpack16<T>(u[b], w);
+      unpack16<T>(u[h], w);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = silu_mul(v[j], w[j]);
-      amax = abs_max16(v);
+      for (int j = 0; j < 16; ++j) v[16 * h + j] = silu_mul(v[16 * h + j], w[j]);
+      amax[h] = abs_max16(v + 16 * h);
     } else {
-      amax = abs_max16(g[b]);
+      amax[h] = abs_max16(g[h]);
     }
-    uint2 c;
-    uint32_t bytes = fp4_quantize16<FMT>(v, amax, q, &c);
-    const int block = static_cast<int>(chunk[b] / kLanes);
-    if (WHOLE) {
-      bytes <<= 8 * (block & 3);
-      bytes |= __shfl_xor_sync(0xffffffffu, bytes, kLanes);
-      bytes |= __shfl_xor_sync(0xffffffffu, bytes, 2 * kLanes);
+  }
+  uint2 c[kHalves];
+  uint32_t bytes;
+  if (FMT == ASHQK_MXFP4) {
+    float d, r;
+    bytes = fp4_scale_of<FMT>(max(amax[0], amax[1]), q, &d, &r);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) c[h] = fp4_codes16<FMT>(v + 16 * h, bytes, d, r);
+  } else {
+    bytes = 0;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      float d, r;
+      const uint32_t byte = fp4_scale_of<FMT>(amax[h], q, &d, &r);
+      c[h] = fp4_codes16<FMT>(v + 16 * h, byte, d, r);
+      bytes |= byte << (8 * h);
     }
-    if (first + b * kQuantThreads >= total) continue;
-    const int64_t r = row0 + row[b];
-    *reinterpret_cast<uint2*>(codes + r * codes_ld + chunk[b] * 8) = c;
-    uint8_t* s = scales + fp4_scale_offset(r, block, tiles);
-    if (WHOLE) {
-      if (chunk[b] % (4 * kLanes) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
-    } else if (chunk[b] % kLanes == 0) {
-      *s = static_cast<uint8_t>(bytes);
-      if (chunk[b] + kLanes == chunks)  // the tile's padding blocks
-        for (int k = block + 1; k & 3; ++k) *++s = 0;
+  }
+  const uint32_t block = chunk * kBlocks;
+  if (WHOLE) {  // the lanes of a tile are neighbours
+    bytes <<= 8 * (block & 3);
+#pragma unroll
+    for (int d = 1; d < 4 / kBlocks; d *= 2) bytes |= __shfl_xor_sync(0xffffffffu, bytes, d);
+  }
+  if (i >= total) return;
+  *reinterpret_cast<uint4*>(codes + row * codes_ld + chunk * (kChunk / 2)) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
+  uint8_t* s = scales + ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+  if (WHOLE) {
+    if ((block & 3) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
+  } else {
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) s[b] = static_cast<uint8_t>(bytes >> (8 * b));
+    if (chunk + 1 == by_chunks.d)  // the tile's padding blocks
+      for (int k = (block & 3) + kBlocks; k < 4; ++k) s[k - (block & 3)] = 0;
+  }
+}
+
+// Rows that start on 16-byte boundaries. One thread: 32 columns, one 16-byte load of codes.
+template <int FMT, typename T>
+__global__ void __launch_bounds__(kQuantThreads)
+    dequantize_rows_kernel(const uint8_t* codes, uint32_t codes_ld, const uint8_t* scales, T* __restrict__ out,
+                           int64_t out_ld, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks, float gs, bool wide) {
+  constexpr int kBlocks = kChunk / fp4_block(FMT);
+  pdl_wait();
+  const uint32_t i = blockIdx.x * kQuantThreads + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t row = divide(i, by_chunks);
+  const uint32_t chunk = i - row * by_chunks.d;
+  const uint32_t block = chunk * kBlocks;
+  const uint4 c4 = ld_once_v4(codes + row * codes_ld + chunk * (kChunk / 2));
+  const uint8_t* s = scales + ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+  const uint32_t bytes = kBlocks == 1 ? *s : *reinterpret_cast<const uint16_t*>(s);
+  const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+  T* y = out + row * out_ld + chunk * kChunk;
+  const int left = K - static_cast<int>(chunk) * kChunk;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // sixteen columns: of one block
+    const float sv = fp4_scale_value<FMT>(kBlocks == 1 ? bytes : (bytes >> (8 * h)) & 0xffu);
+    float v[16];
+    fp4_unpack8(c[2 * h], v);
+    fp4_unpack8(c[2 * h + 1], v + 8);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = v[j] * sv * gs;
+    uint32_t w[4 * sizeof(T)];
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(4 * sizeof(T)); ++j) {
+      if constexpr (sizeof(T) == 2)
+        w[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+      else
+        w[j] = __float_as_uint(v[j]);
+    }
+    T* o = y + 16 * h;
+    const int n = left - 16 * h;
+    if (wide && n >= 16) {
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(4 * sizeof(T)); j += 8)
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(o) + j),
+                     "r"(w[j]), "r"(w[j + 1]), "r"(w[j + 2]), "r"(w[j + 3]), "r"(w[j + 4]), "r"(w[j + 5]), "r"(w[j + 6]), "r"(w[j + 7])
+                     : "memory");
+    } else {
+      constexpr int kPer = 16 / sizeof(T);  // values in 16 bytes
+#pragma unroll
+      for (int j = 0; j < 16; j += kPer) {
+        if (n >= j + kPer)
+          *reinterpret_cast<uint4*>(o + j) = make_uint4(w[4 * (j / kPer)], w[4 * (j / kPer) + 1], w[4 * (j / kPer) + 2], w[4 * (j / kPer) + 3]);
+        else
+#pragma unroll
+          for (int k = 0; k < kPer; ++k)
+            if (j + k < n) o[j + k] = from_f32<T>(v[j + k]);
+      }
     }
   }
 }
 
+// Rows of any alignment. One thread writes eight columns from a 16-byte boundary of the output on: where rows start `mis` values behind one, those are the
+// last `mis` of code word c - 1 and the first of word c (eight codes, all of one block, each).
 template <int FMT, typename T, int BATCH>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_fp4_kernel(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, T* __restrict__ out,
-                          int64_t out_ld, int64_t row0, uint32_t total, int K, FastDiv by_chunks, float gs, bool vec) {
+                          int64_t out_ld, int64_t row0, uint32_t total, int K, FastDiv by_chunks, float gs) {
   pdl_wait();
-  const uint32_t chunks = by_chunks.d;
+  const int words = static_cast<int>(fp4_padded_k(K) / 8);
   const int64_t tiles = fp4_scale_tiles(K, FMT);
   const uint32_t first = blockIdx.x * (kQuantThreads * BATCH) + threadIdx.x;
-  uint32_t c[BATCH], s[BATCH];
+  uint32_t c0[BATCH], c1[BATCH], s0[BATCH], s1[BATCH];
+  int mis[BATCH], word[BATCH];
+  T* o[BATCH];
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) {
     const uint32_t i = first + b * kQuantThreads;
     const uint32_t r = divide(i, by_chunks);
-    const uint32_t chunk = i - r * chunks;
-    c[b] = s[b] = 0;
+    const int c = static_cast<int>(i - r * by_chunks.d);
+    const int64_t row = row0 + r;
+    o[b] = out + row * out_ld;
+    mis[b] = static_cast<int>((reinterpret_cast<uintptr_t>(o[b]) & 15u) / sizeof(T));
+    word[b] = c;
+    c0[b] = c1[b] = s0[b] = s1[b] = 0;
     if (i < total) {
-      c[b] = *reinterpret_cast<const uint32_t*>(codes + (row0 + r) * codes_ld + chunk * 4);
-      s[b] = scales[fp4_scale_offset(row0 + r, static_cast<int>(chunk * 8 / fp4_block(FMT)), tiles)];
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + row * codes_ld);
+      if (c < words) {
+        c1[b] = w[c];
+        s1[b] = scales[fp4_scale_offset(row, c * 8 / fp4_block(FMT), tiles)];
+      }
+      if (mis[b] && c > 0) {
+        c0[b] = w[c - 1];
+        s0[b] = scales[fp4_scale_offset(row, (c - 1) * 8 / fp4_block(FMT), tiles)];
+      }
     }
   }
 #pragma unroll
   for (int b = 0; b < BATCH; ++b) {
-    const uint32_t i = first + b * kQuantThreads;
-    if (i >= total) break;
-    const uint32_t r = divide(i, by_chunks);
-    const int k0 = static_cast<int>(i - r * chunks) * 8;
+    if (first + b * kQuantThreads >= total) break;
+    const int k0 = word[b] * 8 - mis[b];
     float v[8];
-    fp4_unpack8(c[b], v);
-    const float sv = fp4_scale_value<FMT>(s[b]);
+    fp4_unpack8(mis[b] ? __funnelshift_r(c0[b], c1[b], 4 * (8 - mis[b])) : c1[b], v);
+    const float f0 = fp4_scale_value<FMT>(s0[b]), f1 = fp4_scale_value<FMT>(s1[b]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * sv * gs;
-    T* o = out + (row0 + r) * out_ld + k0;
-    if (vec && k0 + 8 <= K) {
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * (j < mis[b] ? f0 : f1) * gs;
+    T* y = o[b] + k0;
+    if (k0 >= 0 && k0 + 8 <= K) {
       if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(o) =
+        *reinterpret_cast<uint4*>(y) =
             make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
       } else {
-        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        reinterpret_cast<float4*>(y)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(y)[1] = make_float4(v[4], v[5], v[6], v[7]);
       }
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (k0 + j < K) o[j] = from_f32<T>(v[j]);
+        if (k0 + j >= 0 && k0 + j < K) y[j] = from_f32<T>(v[j]);
     }
   }
 }
@@ -162,30 +247,28 @@ int launch_pdl(void (*kernel)(Params...), int64_t blocks, int threads, cudaStrea
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...) == cudaSuccess ? ASHQK_OK : ASHQK_ERR_CUDA;
 }
 
-constexpr int kQuantBatch = 2, kDequantBatch = 4;
-// Whether `batch` chunks per thread still leave every SM two blocks (148 SMs).
-constexpr bool many_chunks(int64_t chunks, int batch) { return chunks >= 2 * 148 * kQuantThreads * batch; }
+constexpr int kDequantBatch = 4;
 
-// Calls launch(row0, chunks, blocks of kQuantThreads * batch) for slabs of rows with fewer than 2^31 chunks.
+// Calls launch(row0, rows) for slabs of whole scale tiles with at most `most` rows.
 template <typename F>
-int for_slabs(int64_t rows, int64_t chunks, int batch, F launch) {
-  const int64_t most = std::max<int64_t>(1, ((1ll << 31) - 8 * kQuantThreads) / chunks);
-  for (int64_t row0 = 0; row0 < rows; row0 += most) {
-    const int64_t total = std::min(most, rows - row0) * chunks;
-    if (const int rc = launch(row0, static_cast<uint32_t>(total), ceil_div64(total, kQuantThreads * batch))) return rc;
-  }
+int for_slabs(int64_t rows, int64_t most, F launch) {
+  most = std::max<int64_t>(kFp4TileRows, most / kFp4TileRows * kFp4TileRows);
+  for (int64_t row0 = 0; row0 < rows; row0 += most)
+    if (const int rc = launch(row0, std::min(most, rows - row0))) return rc;
   return ASHQK_OK;
 }
 
-template <int FMT, typename T, bool GATED, int BATCH, bool WHOLE>
+template <int FMT, typename T, bool GATED, bool WHOLE>
 int quantize_launch(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
                     bool early, cudaStream_t stream) {
   int align = chunk_align(x, x_ld, sizeof(T));
   if (GATED) align = std::min(align, chunk_align(nullptr, K, sizeof(T)));
-  const int64_t chunks = fp4_padded_k(K) / 16;
-  return for_slabs(M, chunks, BATCH, [&](int64_t row0, uint32_t total, int64_t blocks) {
-    return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, BATCH, WHOLE>, blocks, kQuantThreads, stream,
-                      static_cast<const T*>(x), x_ld, codes, codes_ld, scales, row0, total, K,
+  const int64_t chunks = fp4_padded_k(K) / kChunk;
+  const int64_t tiles = fp4_scale_tiles(K, FMT);
+  return for_slabs(M, ((1ll << 31) - 1) / codes_ld, [&](int64_t row0, int64_t rows) {
+    return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, WHOLE>, ceil_div64(rows * chunks, kQuantThreads), kQuantThreads,
+                      stream, static_cast<const T*>(x) + row0 * x_ld, x_ld, codes + row0 * codes_ld, codes_ld,
+                      scales + row0 / kFp4TileRows * tiles * kFp4TileBytes, tiles, rows * chunks, K,
                       fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(gs), align, early);
   });
 }
@@ -193,12 +276,9 @@ int quantize_launch(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_l
 template <int FMT, typename T, bool GATED>
 int quantize_shaped(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
                     bool early, cudaStream_t stream) {
-  const int64_t kp = fp4_padded_k(K);
-  const bool whole = kp % (4 * fp4_block(FMT)) == 0;
-  const bool many = many_chunks(M * (kp / 16), kQuantBatch);
-  return (whole ? many ? quantize_launch<FMT, T, GATED, kQuantBatch, true> : quantize_launch<FMT, T, GATED, 1, true>
-          : many ? quantize_launch<FMT, T, GATED, kQuantBatch, false>
-                 : quantize_launch<FMT, T, GATED, 1, false>)(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
+  const bool whole = fp4_padded_k(K) % (4 * fp4_block(FMT)) == 0;
+  return (whole ? quantize_launch<FMT, T, GATED, true> : quantize_launch<FMT, T, GATED, false>)(
+      x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
 }
 
 template <int FMT, typename T>
@@ -211,13 +291,23 @@ int quantize_typed(const void* x, int64_t x_ld, bool gated, uint8_t* codes, int6
 template <int FMT, typename T>
 int dequantize_typed(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, void* out, int64_t out_ld, int M,
                      int K, float gs, cudaStream_t stream) {
-  const bool vec = aligned(out, 16) && (out_ld * sizeof(T)) % 16 == 0;
-  const int64_t chunks = (K + 7) / 8;
-  const bool many = many_chunks(M * chunks, kDequantBatch);
-  return for_slabs(M, chunks, many ? kDequantBatch : 1, [&](int64_t row0, uint32_t total, int64_t blocks) {
-    return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kDequantBatch> : dequantize_fp4_kernel<FMT, T, 1>, blocks,
-                      kQuantThreads, stream, codes, codes_ld, scales, static_cast<T*>(out), out_ld, row0, total, K,
-                      fast_div(static_cast<uint32_t>(chunks)), gs, vec);
+  if (const int align = chunk_align(out, out_ld, sizeof(T))) {
+    const int64_t chunks = ceil_div64(K, kChunk);
+    const int64_t tiles = fp4_scale_tiles(K, FMT);
+    return for_slabs(M, ((1ll << 31) - 1) / codes_ld, [&](int64_t row0, int64_t rows) {
+      return launch_pdl(dequantize_rows_kernel<FMT, T>, ceil_div64(rows * chunks, kQuantThreads), kQuantThreads, stream,
+                        codes + row0 * codes_ld, codes_ld, scales + row0 / kFp4TileRows * tiles * kFp4TileBytes,
+                        static_cast<T*>(out) + row0 * out_ld, out_ld, tiles, rows * chunks, K,
+                        fast_div(static_cast<uint32_t>(chunks)), gs, align == 32);
+    });
+  }
+  const int64_t chunks = (K + 7) / 8 + 1;  // a row that starts off a boundary may touch one more
+  return for_slabs(M, ((1ll << 31) - 8 * kQuantThreads) / chunks, [&](int64_t row0, int64_t rows) {
+    const int64_t total = rows * chunks;
+    const bool many = total >= 2 * 148 * kQuantThreads * kDequantBatch;  // every SM (of 148) still gets two blocks
+    return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kDequantBatch> : dequantize_fp4_kernel<FMT, T, 1>,
+                      ceil_div64(total, kQuantThreads * (many ? kDequantBatch : 1)), kQuantThreads, stream, codes, codes_ld,
+                      scales, static_cast<T*>(out), out_ld, row0, total, K, fast_div(static_cast<uint32_t>(chunks)), gs);
   });
 }
 

@@ -105,6 +105,44 @@ def test_dequantize_exact(fmt, dtype, m, k):
     assert got.shape == (m, k) and torch.equal(got.cpu(), want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [0, 1, 2], ids=["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("start", [0, 1, 3, 4, 8])
+def test_dequantize_into_rows_of_any_alignment(fmt, dtype, start):
+    """Rows that start anywhere, of any pitch; what lies between and behind them stays as it was."""
+    import ctypes
+
+    from ashqk import _ext
+
+    lib = ctypes.CDLL(_ext.C_LIBRARY)
+    vp, i64, ci = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+    lib.ashqk_dequantize_fp4.argtypes = [vp, i64, vp, vp, i64, ci, ci, ci, ci, ctypes.c_float, vp]
+    t = (torch.float16, torch.bfloat16, torch.float32)[dtype]
+    for k, ld in ((1, 1), (7, 11), (32, 33), (100, 104), (250, 256), (333, 335), (1024, 1030)):
+        q, v64 = random_operand(5, k, fmt, k)
+        buf = torch.full((start + 6 * ld,), 9.0, dtype=t, device="cuda")
+        out = buf[start : start + 5 * ld].view(5, ld)
+        rc = lib.ashqk_dequantize_fp4(q.codes.data_ptr(), q.codes.stride(0), q.scales.data_ptr(), out.data_ptr(), ld, dtype, 5, k,
+                                      FORMATS.index(fmt), 1.0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert torch.equal(out[:, :k], v64.to(t)), (k, ld)
+        out[:, :k] = 9.0
+        assert bool((buf == 9.0).all()), (k, ld)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_quantize_rows_of_any_alignment(fmt, dtype):
+    base = rows(9, 700, dtype, 3)
+    for start, k in ((1, 32), (2, 97), (3, 640), (4, 15), (5, 333), (6, 16), (7, 48), (8, 500), (9, 31)):
+        x = base[:, start : start + k]
+        check_quantised(ashqk.quantize_fp4(x, fmt, global_scale=G[fmt]), x.double().cpu().numpy(), fmt, G[fmt], 9, k)
+        if dtype != "fp32":
+            w, w64 = random_operand(40, k, fmt, k)
+            a, b = ashqk.w4a4_linear(x, w, global_scale=G[fmt]), ashqk.w4a4_linear(x.contiguous(), w, global_scale=G[fmt])
+            assert torch.equal(a, b), (start, k)
+
+
 def test_dequantize_mxfp4_extreme_scales():
     code = np.tile(np.arange(16, dtype=np.uint8), (256, 2))
     byte = np.arange(256, dtype=np.uint8)[:, None]
