@@ -13,8 +13,8 @@
 //   warp 1      one elected lane: tcgen05.cp of a stage's scales, its four MMAs, commit
 //   warps 2..9  fused form: quantise this CTA's slice of A into shared memory, in the layout in which TMA and
 //               the scale tiles arrive otherwise; then all: TMEM -> registers -> y, or, with a split K,
-//               -> the shared memory of the CTA that adds these rows of A (st.async, counted in bytes on
-//               its barrier)
+//               -> the shared memory of the CTA that adds these rows of A, counted in bytes on its barrier
+//               (st.async, or with 32 columns and more through own shared memory and bulk copies)
 //
 // The scales' TMEM columns are double-buffered: stage i's copies wait for the MMAs of stage i - 2. All
 // waits are bounded.
@@ -24,6 +24,9 @@
 #include "fp4_mma.cuh"
 
 namespace ashqk {
+
+void fp4_set_pair_split(int split);
+
 namespace {
 
 constexpr int kTileN = 128;  // weight rows per CTA
@@ -55,37 +58,30 @@ struct RowsArgs {
 template <int FMT, int NT, bool FUSED>
 struct RowsShape {
   static constexpr int kT = Fp4Mma<FMT>::kTilesPerStage;
-  static constexpr int kXTiles = NT > 128 ? 2 : 1;  // 128-row scale tiles of A's rows
   static constexpr uint32_t kW = kTileN * 128;
   static constexpr uint32_t kWS = kT * kFp4TileBytes;
   static constexpr uint32_t kX = NT * 128;
-  static constexpr uint32_t kXS = kXTiles * kT * kFp4TileBytes;
+  static constexpr uint32_t kXS = kT * kFp4TileBytes;
   static constexpr uint32_t kStage = kW + kWS + (FUSED ? 0 : kX + kXS);
   static_assert(kStage % 1024 == 0, "swizzle atoms need 1 KB alignment");
   // Fused: the quantised slice, [stage][row][128] and after it the scale tiles, of which only the first NT rows
   // are there: the copy to TMEM reads on into the next tile, for rows that nobody uses.
   static constexpr uint32_t kXSTile = NT * 16;
   // TMEM: the sums, then two buffers of scales.
-  static constexpr int kSfW = kT * 4, kSfX = kXTiles * kT * 4;
+  static constexpr int kSfW = kT * 4, kSfX = kT * 4;
   static constexpr int kSf0 = NT < 32 ? 32 : NT;
   static constexpr int kCols = kSf0 + 2 * (kSfW + kSfX);
-  static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
-  static_assert(kCols <= 512, "TMEM");
-  // Split K: whether the slots for partial sums have shared memory of their own or take the ring's.
+  static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
+  static_assert(kCols <= 256, "TMEM");
+  // Split K: whether the slots for partial sums have shared memory of their own or take the ring's, and whether
+  // the sums go there by way of the own ring.
   static constexpr bool kOwnSlots = NT <= 32;
+  static constexpr bool kStaged = NT >= 32;
+  static constexpr uint32_t kStaging = NT / 4 * kTileN * 16;
   static constexpr uint32_t slots(int cluster) {
     return static_cast<uint32_t>(((NT / 4 + cluster - 1) / cluster) * cluster) * kTileN * 16;
   }
 };
-
-__device__ __forceinline__ void st_async_v4(uint32_t remote_addr, uint4 v, uint32_t remote_bar) {
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(
-                   remote_addr),
-               "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(remote_bar)
-               : "memory");
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
@@ -197,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     mbar_init(received, 1);
     *abort = 0;
     fence_mbarrier_init();
-    if (C > 1) mbar_arrive_expect_tx(received, static_cast<uint32_t>(my_groups * C) * kTileN * 16);
+    if (C > 1) mbar_arrive_expect_tx(received, static_cast<uint32_t>(my_groups * (C - 1)) * kTileN * 16);
   }
   __syncthreads();
   // This CTA's barriers can be signalled (waited for before the first remote store). Before the allocation, which
@@ -227,7 +223,6 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   const uint32_t x_scales = x_codes + static_cast<uint32_t>(kb1 - kb0) * L::kX;
 
   if (warp == 0) {
-    const int x_tiles = FUSED ? 0 : min(L::kXTiles, (a.M - m0 + 127) / 128);
     int stage = 0;
     uint32_t phase = 0;
     int issued = 0;
@@ -237,14 +232,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
       const int t0 = kb * L::kT;
       const uint32_t sf = static_cast<uint32_t>(min(L::kT, a.scale_tiles - t0)) * kFp4TileBytes;
       if (elect_one()) {
-        mbar_arrive_expect_tx(&full[stage], L::kW + (FUSED ? 0 : L::kX) + sf * (1 + x_tiles));
+        mbar_arrive_expect_tx(&full[stage], L::kW + sf + (FUSED ? 0 : L::kX + sf));
         tma_load_2d(base, &maps.w, kb * 128, n0, &full[stage]);
         bulk_load(base + L::kW, a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
         if (!FUSED) {
           tma_load_2d(base + L::kW + L::kWS, &maps.x, kb * 128, m0, &full[stage]);
-          for (int t = 0; t < x_tiles; ++t)
-            bulk_load(base + L::kW + L::kWS + L::kX + t * L::kWS,
-                      a.xs + (static_cast<int64_t>(m0 / 128 + t) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+          bulk_load(base + L::kW + L::kWS + L::kX, a.xs + (static_cast<int64_t>(m0 / kFp4TileRows) * a.scale_tiles + t0) * kFp4TileBytes,
+                    sf, &full[stage]);
         }
       }
       __syncwarp();
@@ -293,19 +287,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         for (int t = 0; t < L::kT; ++t) {
           if (t >= tiles) break;
           scale_tile_to_tmem(sfw + t * 4, sd + t * (kFp4TileBytes >> 4));
-          if (FUSED) {
-            scale_tile_to_tmem(sfx + t * 4, sx + t * (L::kXSTile >> 4));
-          } else {
-#pragma unroll
-            for (int r = 0; r < L::kXTiles; ++r)
-              scale_tile_to_tmem(sfx + (t * L::kXTiles + r) * 4, sx + ((r * L::kWS + t * kFp4TileBytes) >> 4));
-          }
+          scale_tile_to_tmem(sfx + t * 4, sx + t * ((FUSED ? L::kXSTile : kFp4TileBytes) >> 4));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (j >= steps) break;
           Mma::mma(tmem, dw + 2 * j, dx + 2 * j, Mma::idesc(kTileN, NT, j), sfw + Mma::tile_of(j) * 4,
-                   sfx + Mma::tile_of(j) * L::kXTiles * 4, (i | j) != 0);
+                   sfx + Mma::tile_of(j) * 4, (i | j) != 0);
         }
         umma_commit(&empty[stage]);
         if (kb + 1 == kb1) umma_commit(done);
@@ -349,15 +337,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     ok = mbar_wait(done, 0, abort);
     tc_fence_after_sync();
   }
-  if (C > 1) {
+  // Slots: [group of this rank][sender][weight row] x 16 bytes. Staging: [group][weight row] x 16 bytes.
+  const uint32_t slots = sbase + (L::kOwnSlots ? a.off_slots : L::kStaging);
+  auto slot = [&](int l, int from) { return slots + static_cast<uint32_t>((l * C + from) * kTileN + row) * 16; };
+  if (C > 1 && !L::kStaged) {
     __syncwarp();
     cluster_wait();
-    if (!L::kOwnSlots) {  // every CTA of the cluster is through with its ring
-      __syncthreads();
-      cluster_sync();
-    }
   }
-  const uint32_t slots = sbase + (L::kOwnSlots ? a.off_slots : 0u);
   // Four sums of consecutive rows of A -> y. Lanes are consecutive columns of y: 64 bytes per row and warp.
   auto store4 = [&](int m, float v0, float v1, float v2, float v3) {
     if (n >= a.N) return;
@@ -393,17 +379,21 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
                  __uint_as_float(r[4 * h + 3]));
         } else {
           const int l = g / C, owner = g - l * C;
-          const uint32_t at = slots + static_cast<uint32_t>((l * C + rank) * kTileN + row) * 16;
-          uint32_t remote, bar;
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(at), "r"(owner));
-          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(received)), "r"(owner));
-          st_async_v4(remote, make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]), bar);
+          const uint4 v = make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]);
+          if (owner == rank && (L::kOwnSlots || !L::kStaged))
+            sts_v4(slot(l, rank), v);
+          else if (L::kStaged)
+            sts_v4(sbase + static_cast<uint32_t>(g * kTileN + row) * 16, v);
+          else
+            st_async_v4(map_rank(slot(l, rank), owner), v, map_rank(smem_u32(received), owner));
         }
       }
     }
   }
   tc_fence_before_sync();
   __syncthreads();
+  // TMEM goes back before the CTA waits for its cluster: a CTA that holds it waits for nobody, so CTAs of
+  // several clusters that share SMs cannot block one another in the allocation.
   if (warp == 1) {
     __syncwarp();
     tc_fence_after_sync();
@@ -411,6 +401,24 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   }
   if (C > 1) {
     __syncwarp();
+    if (L::kStaged) {
+      cluster_wait();
+      if (!L::kOwnSlots) cluster_sync();  // every CTA of the cluster is through with its ring
+      if (epilogue) {  // each warp sends the 512 bytes of every group that it has written
+        constexpr int kPer = 8;  // groups of one TMEM load
+        fence_proxy_async_smem();
+        __syncwarp();
+        for (int i = lane; i < (groups + kPer - 1) / kPer * kPer; i += 32) {
+          const int g = i, l = g / C, owner = g - l * C;
+          if (g < groups && ((g / kPer) & 1) == turn && owner != rank) {
+            const uint32_t first = static_cast<uint32_t>(row - lane) * 16;
+            bulk_to_cluster(map_rank(slots + static_cast<uint32_t>((l * C + rank) * kTileN) * 16 + first, owner),
+                            sbase + static_cast<uint32_t>(g * kTileN) * 16 + first, 512, map_rank(smem_u32(received), owner));
+          }
+        }
+        __syncwarp();
+      }
+    }
     cluster_arrive();
     if (epilogue && my_groups > 0 && mbar_wait_cluster(received, 0, abort)) {
 #pragma unroll 2
@@ -418,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int c = 0; c < C; ++c) {
-          const uint4 p = lds_v4(slots + static_cast<uint32_t>((l * C + c) * kTileN + row) * 16);
+          // without slots of its own, this CTA's sums are still where they were staged
+          const uint4 p = lds_v4(!L::kOwnSlots && c == rank ? sbase + static_cast<uint32_t>((l * C + rank) * kTileN + row) * 16 : slot(l, c));
           s[0] += __uint_as_float(p.x), s[1] += __uint_as_float(p.y), s[2] += __uint_as_float(p.z), s[3] += __uint_as_float(p.w);
         }
         store4(m0 + 4 * (l * C + rank), s[0], s[1], s[2], s[3]);
@@ -447,9 +456,10 @@ template <int FMT, int NT, bool FUSED>
 RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   using L = RowsShape<FMT, NT, FUSED>;
   RowsPlan p;
-  // Wide tiles without slots of their own have an SM to themselves, and clusters of such CTAs do not fill every SM.
-  const int ctas = L::kTmemCols > 128 ? sm_count * 9 / 10 : sm_count * 27 / 20;
-  p.cluster = std::max(1, std::min({kMaxCluster, num_kb, ctas / std::max(1, tiles)}));
+  // 128 rows of A: the staged sums leave room for one CTA per SM, and clusters of those do not fill every SM (2048
+  // columns of K and rows of B in clusters of eight: 15.8 us in two waves).
+  const int ctas = NT > 64 ? sm_count * 9 / 10 : sm_count * 27 / 20;
+  p.cluster = std::max(1, std::min({NT > 64 ? 4 : kMaxCluster, num_kb, ctas / std::max(1, tiles)}));
   if (p.cluster == 1 && L::kOwnSlots && num_kb >= 4 && tiles > sm_count && tiles <= ctas) p.cluster = 2;
   auto x_area = [&] {  // this CTA's slice of A, quantised
     return FUSED ? ceil_div(num_kb, p.cluster) * (L::kX + L::kT * L::kXSTile) + kFp4TileBytes : 0u;
@@ -460,23 +470,18 @@ RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   const uint32_t x_bytes = x_area();
   const uint32_t slots = p.cluster > 1 ? L::slots(p.cluster) : 0;
   // Shared memory for the ring: a third of an SM for narrow tiles that split K (this launch's CTAs and the next's
-  // are resident together), half of one otherwise, all of it for 512 TMEM columns.
-  const uint32_t budget = (L::kTmemCols > 256 ? 218 : L::kOwnSlots && p.cluster > 1 ? 72 : 108) * 1024;
+  // are resident together), half of one otherwise.
+  const uint32_t budget = (L::kOwnSlots && p.cluster > 1 ? 72 : 108) * 1024;
   const uint32_t fixed = x_bytes + (L::kOwnSlots ? slots : 0);
   p.ring = fixed + 2 * L::kStage > budget ? 2 : static_cast<int>((budget - fixed) / L::kStage);
   p.ring = std::max(2, std::min({kMaxRing, local, p.ring}));
   if (const int r = g_ring.load(std::memory_order_relaxed)) p.ring = std::max(2, std::min({r, local, static_cast<int>((222 * 1024 - std::min(fixed, 222u * 1024)) / L::kStage)}));
   uint32_t ring = p.ring * L::kStage;
-  if (!L::kOwnSlots) ring = std::max(ring, (slots + 1023) / 1024 * 1024);
+  if (p.cluster > 1 && L::kStaged) ring = std::max(ring, (L::kStaging + (L::kOwnSlots ? 0 : slots) + 1023) / 1024 * 1024);
   p.off_x = ring;
   p.off_slots = (p.off_x + x_bytes + 15) / 16 * 16;
   p.off_bar = (p.off_slots + (L::kOwnSlots ? slots : 0) + 7) / 8 * 8;
   p.smem = p.off_bar + (2 * kMaxRing + 3) * 8 + 16 + 1024;
-  // Without slots of their own, the CTAs of a cluster wait for one another while they hold TMEM. Two such CTAs on
-  // one SM must therefore both fit its 512 columns, or clusters could wait for each other's allocation in a
-  // circle: 128 columns always do (registers hold an SM to three CTAs), 256 are one to an SM, 512 alone.
-  if (!L::kOwnSlots && p.cluster > 1)
-    p.smem = std::max(p.smem, L::kTmemCols <= 128 ? 0u : L::kTmemCols == 256 ? 116u * 1024 : 200u * 1024);
   return p;
 }
 
@@ -526,8 +531,7 @@ int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, bool fused,
     case 16: return launch_rows<FMT, 16, false>(maps, a, stream);
     case 32: return launch_rows<FMT, 32, false>(maps, a, stream);
     case 64: return launch_rows<FMT, 64, false>(maps, a, stream);
-    case 128: return launch_rows<FMT, 128, false>(maps, a, stream);
-    default: return launch_rows<FMT, 256, false>(maps, a, stream);
+    default: return launch_rows<FMT, 128, false>(maps, a, stream);
   }
 }
 
@@ -554,7 +558,7 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
                     const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
                     cudaStream_t stream) {
   int nt = 8;
-  while (nt < M && nt < 256) nt *= 2;
+  while (nt < M && nt < 128) nt *= 2;
   RowsMaps maps;
   RowsArgs a = {};
   int rc = rows_args(a, maps, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N, K, format, alpha);
@@ -596,9 +600,11 @@ int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_
 
 }  // namespace ashqk
 
-extern "C" int ashqk_fp4_set_tuning(int cluster, int ring) {
+extern "C" int ashqk_fp4_set_tuning(int cluster, int ring, int split) {
+  if (split < 0 || split > 2) return ASHQK_ERR_INVALID_ARGUMENT;
   if (cluster < 0 || cluster > ashqk::kMaxCluster || ring < 0 || ring == 1 || ring > ashqk::kMaxRing) return ASHQK_ERR_INVALID_ARGUMENT;
   ashqk::g_cluster.store(cluster, std::memory_order_relaxed);
   ashqk::g_ring.store(ring, std::memory_order_relaxed);
+  ashqk::fp4_set_pair_split(split);
   return ASHQK_OK;
 }

@@ -27,6 +27,12 @@ namespace {
 
 std::atomic<int> g_matmul_kernel{0};
 
+// Few rows go to the rows kernel, whose CTAs split K, the others to CTA pairs. Measured in graphs (MXFP4, us, rows
+// against pairs): 64 rows 8.2 / 9.4 (4096->6144), 7.9 / 9.1 (4096->4096), 10.9 / 14.9 (12288->4096), 15.2 / 17.6
+// (4096->24576); 128 rows 10.5 / 9.9, 9.0 / 9.6, 13.8 / 15.2, 17.6 / 18.7; 256 rows 10.9 / 9.9, 10.8 / 9.6,
+// 18.2 / 15.2. Between 64 and 128 rows it is the number of tiles that decides: the fewer, the finer the split of K.
+bool few_rows(int M, int N) { return M <= 64 || (M <= 128 && N <= 5120); }
+
 // Q(x) in the workspace: scales first (a multiple of 512 bytes), then codes.
 void workspace_layout(int M, int K, int format, size_t* codes_offset, size_t* bytes) {
   *codes_offset = static_cast<size_t>(ceil_div64(M, kFp4TileRows) * fp4_scale_tiles(K, format) * kFp4TileBytes);
@@ -52,7 +58,7 @@ extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a
   if (const int rc = check_fp4_operand(a_codes, a_ld, a_scales, K)) return rc;
   if (const int rc = check_fp4_operand(b_codes, b_ld, b_scales, K)) return rc;
   const int which = g_matmul_kernel.load(std::memory_order_relaxed);
-  const bool pair = which ? which == 2 : M > 128;
+  const bool pair = which ? which == 2 : !few_rows(M, N);
   return (pair ? fp4_matmul_pair : fp4_matmul_rows)(a_codes, a_ld, a_scales, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N,
                                                     K, format, alpha, static_cast<cudaStream_t>(stream));
 }

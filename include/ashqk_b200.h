@@ -373,15 +373,15 @@ ASHQK_API int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gate
 
 /*
  * Tuning and test switch (process-wide): which product kernel the two calls above use. 0 automatic,
- * 1 rows (128 rows of B by up to 256 of A per CTA, K split over a cluster), 2 CTA pairs (256 x 256).
+ * 1 rows (128 rows of B by up to 128 of A per CTA, K split over a cluster), 2 CTA pairs (256 x 256).
  */
 ASHQK_API int ashqk_set_fp4_kernel(int which);
 
 /*
- * The same for the rows kernel's plan: CTAs per cluster (up to 8) and stages in flight (2 to 12) instead of the
- * automatic ones; 0 restores them.
+ * The same for the kernels' plans, instead of the automatic ones; 0 restores them. rows kernel: CTAs per cluster (up
+ * to 8) and stages in flight (2 to 12); pair kernel: pairs per tile, K split (1, or 2 where that many are resident).
  */
-ASHQK_API int ashqk_fp4_set_tuning(int cluster, int ring);
+ASHQK_API int ashqk_fp4_set_tuning(int cluster, int ring, int split);
 
 #ifdef __cplusplus
 }

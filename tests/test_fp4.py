@@ -145,7 +145,9 @@ def test_c_abi_switches():
     for which, want in ((0, 0), (1, 0), (2, 0), (3, 1), (-1, 1), (0, 0)):
         assert lib.ashqk_set_fp4_kernel(which) == want
     for cluster, ring, want in ((1, 2, 0), (8, 12, 0), (9, 2, 1), (-1, 0, 1), (0, 1, 1), (0, 13, 1), (0, -1, 1), (0, 0, 0)):
-        assert lib.ashqk_fp4_set_tuning(cluster, ring) == want
+        assert lib.ashqk_fp4_set_tuning(cluster, ring, 0) == want
+    for split, want in ((1, 0), (2, 0), (3, 1), (4, 1), (-1, 1), (0, 0)):
+        assert lib.ashqk_fp4_set_tuning(0, 0, split) == want
 
 
 def _refusals(good: dict, bad: list):

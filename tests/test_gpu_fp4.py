@@ -340,7 +340,7 @@ def test_every_split_of_k(cluster, ring, fmt):
     from ashqk import _ext
 
     lib = ctypes.CDLL(_ext.C_LIBRARY)
-    assert lib.ashqk_fp4_set_tuning(cluster, ring) == 0 and lib.ashqk_set_fp4_kernel(1) == 0
+    assert lib.ashqk_fp4_set_tuning(cluster, ring, 0) == 0 and lib.ashqk_set_fp4_kernel(1) == 0
     try:
         for m, n, k in ((1, 300, 2080), (4, 128, 4096), (13, 256, 1500), (30, 200, 2304), (61, 130, 1024), (100, 128, 2080), (200, 256, 1056), (300, 140, 800)):
             b, b64 = random_operand(n, k, fmt, n)
@@ -352,7 +352,28 @@ def test_every_split_of_k(cluster, ring, fmt):
                 x64 = torch.from_numpy(F.values(code, byte, fmt, G[fmt])[:, :k]).cuda()
                 check_product(ashqk.w4a4_linear(x, b, global_scale=G[fmt]), x64, b64, 2.0**-23)
     finally:
-        assert lib.ashqk_fp4_set_tuning(0, 0) == 0 and lib.ashqk_set_fp4_kernel(0) == 0
+        assert lib.ashqk_fp4_set_tuning(0, 0, 0) == 0 and lib.ashqk_set_fp4_kernel(0) == 0
+
+
+@pytest.mark.parametrize("split", [1, 2])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_pairs_that_split_k(split, fmt):
+    """Pair tiles whose K is taken by one pair or two: even and uneven shares, ragged edges, an odd pitch of y."""
+    import ctypes
+
+    from ashqk import _ext
+
+    lib = ctypes.CDLL(_ext.C_LIBRARY)
+    assert lib.ashqk_fp4_set_tuning(0, 0, split) == 0 and lib.ashqk_set_fp4_kernel(2) == 0
+    try:
+        for m, n, k in ((256, 256, 1024), (130, 500, 4096), (300, 777, 2400), (1, 24, 1100), (512, 1024, 1300), (250, 256, 12288), (700, 300, 5 * 256)):
+            a, a64 = random_operand(m, k, fmt, m)
+            b, b64 = random_operand(n, k, fmt, n)
+            y = ashqk.fp4_matmul(a, b)
+            check_product(y, a64, b64)
+            assert torch.equal(ashqk.fp4_matmul(a, b), y)
+    finally:
+        assert lib.ashqk_fp4_set_tuning(0, 0, 0) == 0 and lib.ashqk_set_fp4_kernel(0) == 0
 
 
 def test_empty():
