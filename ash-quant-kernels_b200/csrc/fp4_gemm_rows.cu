@@ -1,5 +1,5 @@
 // y = alpha * A B^T with 4-bit operands, for any number of rows of A; made for few. A comes quantised, or
-// (up to 16 rows) in 16 bits and is quantised here.
+// (up to 32 rows) in 16 bits and is quantised here.
 //
 // The weights' rows (B, N of them) take the tensor core's 128-row side and A's rows its column side, so that
 // one token wastes 7 of 8 columns instead of 127 of 128 rows, and every weight byte goes from HBM
@@ -525,7 +525,10 @@ int launch_rows(const RowsMaps& maps, RowsArgs a, cudaStream_t stream) {
 
 template <int FMT>
 int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, bool fused, cudaStream_t stream) {
-  if (fused) return nt == 8 ? launch_rows<FMT, 8, true>(maps, a, stream) : launch_rows<FMT, 16, true>(maps, a, stream);
+  if (fused)
+    return nt == 8    ? launch_rows<FMT, 8, true>(maps, a, stream)
+           : nt == 16 ? launch_rows<FMT, 16, true>(maps, a, stream)
+                      : launch_rows<FMT, 32, true>(maps, a, stream);
   switch (nt) {
     case 8: return launch_rows<FMT, 8, false>(maps, a, stream);
     case 16: return launch_rows<FMT, 16, false>(maps, a, stream);
@@ -571,13 +574,15 @@ int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, con
                                : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, false, stream);
 }
 
-// Whether w4a4_linear quantises x inside the product: up to 16 rows, of a length whose slice fits beside the ring (an
-// eighth of 32768 columns: 16 stages of at most 3 KB), and where every 128 weight rows quantising x anew costs
-// less than a launch for it. Measured (MXFP4, fused against two launches, in a graph): at M K tiles = 6.3 million
-// 12.8 against 15.9 us (8 rows 4096->24576) and 11.2 against 11.7 (16 rows 12288->4096), at 12.6 million 15.3
-// against 16.1 (16 rows 4096->24576; NVFP4 17.2 against 17.2).
+// Whether w4a4_linear quantises x inside the product: up to 32 rows, of a length whose slice fits beside the ring (an
+// eighth of it at most 48 KB), and where every 128 weight rows quantising x anew costs less than a launch for it.
+// Measured (us, fused against two launches, in a graph): up to 16 rows, at M K tiles = 6.3 million 12.8 / 15.9
+// (8 rows 4096->24576) and 11.2 / 11.7 (16 rows 12288->4096), at 12.6 million 15.3 / 16.1 (16 rows 4096->24576;
+// NVFP4 17.2 / 17.2); with the wider instruction of 32 rows 8.4 / 9.3 at 4.2 million (4096->4096), 9.8 / 9.9 at 6.3
+// million (4096->6144), 13.2 / 12.7 at 9.4 million (24 rows 12288->4096).
 bool fp4_fused_ok(int M, int N, int K) {
-  return M <= 16 && K <= 32768 && static_cast<int64_t>(M) * K * ceil_div(N, kTileN) <= (1 << 24);
+  const int64_t work = static_cast<int64_t>(M) * K * ceil_div(N, kTileN);
+  return M <= 16 ? K <= 32768 && work <= (1 << 24) : M <= 32 && K <= 16384 && work <= (6 << 20);
 }
 
 int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
@@ -593,7 +598,7 @@ int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_
   a.xq = fp4_quant_params(x_gs);
   a.gated = gated;
   a.align = std::min(chunk_align(x, x_ld, 2), gated ? chunk_align(nullptr, K, 2) : 32);
-  const int nt = M <= 8 ? 8 : 16;
+  const int nt = M <= 8 ? 8 : M <= 16 ? 16 : 32;
   return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, true, stream)
                                : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, true, stream);
 }
