@@ -18,6 +18,7 @@ from typing import Dict, Iterable, Optional
 
 import torch
 
+from .fp4 import FP4Linear
 from .ops import w4a16_linear
 
 _SUFFIXES = ("qweight", "qzeros", "scales")
@@ -175,8 +176,11 @@ class AWQLinear(torch.nn.Module):
                 f"group_size={self.in_features // self.scales.shape[0]}, bias={self.bias is not None}")
 
 
-def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer]) -> list[str]:
+def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer], fp4_format: Optional[str] = None) -> list[str]:
     """Swap each ``nn.Linear`` of ``model`` named in ``layers`` for an ``AWQLinear``.
+
+    With ``fp4_format`` ("mxfp4" or "nvfp4") for an ``FP4Linear`` instead: the checkpoint's weights, quantised again
+    to 4-bit floating point, times activations quantised as they come (layers on the GPU).
 
     Names follow ``model.named_modules()``. The quantised layer must have the Linear's in/out
     features. Returns the replaced names; layers of the checkpoint that match no module are an error.
@@ -195,6 +199,6 @@ def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer]) -
                              f"{mod.in_features}->{mod.out_features}")
         parent_name, _, child = name.rpartition(".")
         parent = modules[parent_name] if parent_name else model
-        setattr(parent, child, AWQLinear.from_layer(layer))
+        setattr(parent, child, FP4Linear.from_awq(layer, fp4_format) if fp4_format else AWQLinear.from_layer(layer))
         replaced.append(name)
     return replaced

@@ -161,3 +161,54 @@ def w4a4_linear(x: torch.Tensor, weight: FP4Tensor, *, global_scale: float = 1.0
     _check_global_scale(weight.format, global_scale)
     return _op("w4a4_linear")(x, weight.codes, weight.scales, weight.shape[1], _format(weight.format), global_scale,
                               weight.global_scale, gated)
+
+
+class FP4Linear(torch.nn.Module):
+    """A linear layer y = Q(x) @ W^T (+ bias) with W [out, in] held as an ``FP4Tensor``; CUDA only.
+
+    The W4A4 counterpart of ``AWQLinear``. ``input_global_scale`` is x's, for "nvfp4"; ``gated`` as in ``w4a4_linear``.
+    """
+
+    def __init__(self, weight: FP4Tensor, bias: torch.Tensor | None = None, *, input_global_scale: float = 1.0, gated: bool = False):
+        super().__init__()
+        _check_global_scale(weight.format, input_global_scale)
+        assert bias is None or bias.shape == (weight.shape[0],), f"bias {tuple(bias.shape)} for {weight.shape[0]} outputs"
+        self.register_buffer("codes", weight.codes)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("bias", bias)
+        self.out_features, self.in_features = weight.shape
+        self.format, self.global_scale = weight.format, weight.global_scale
+        self.input_global_scale, self.gated = input_global_scale, gated
+
+    @staticmethod
+    def from_float(weight: torch.Tensor, bias: torch.Tensor | None = None, format: str = "nvfp4", **kwargs) -> "FP4Linear":
+        """From a dense weight [out, in] on the GPU; for "nvfp4" the global scale is ``fp4_global_scale(weight)``."""
+        g = fp4_global_scale(weight) if format == "nvfp4" else 1.0
+        return FP4Linear(quantize_fp4(weight.detach(), format, global_scale=g), bias, **kwargs)
+
+    @staticmethod
+    def from_awq(layer, format: str = "nvfp4", **kwargs) -> "FP4Linear":
+        """From an ``AWQLayer`` on the GPU: its int4 weights are dequantised to fp16 and quantised again."""
+        w = _op("dequantize_awq")(layer.qweight, layer.qzeros, layer.scales, torch.float16)
+        return FP4Linear.from_float(w.t(), layer.bias, format, **kwargs)
+
+    @property
+    def weight(self) -> FP4Tensor:
+        return FP4Tensor(self.codes, self.scales, (self.out_features, self.in_features), self.format, self.global_scale)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = w4a4_linear(x, self.weight, global_scale=self.input_global_scale, gated=self.gated)
+        return y + self.bias.to(y.dtype) if self.bias is not None else y
+
+    def get_extra_state(self):
+        return {"format": self.format, "shape": (self.out_features, self.in_features), "global_scale": self.global_scale,
+                "input_global_scale": self.input_global_scale}
+
+    def set_extra_state(self, state) -> None:
+        assert tuple(state["shape"]) == (self.out_features, self.in_features) and state["format"] == self.format, \
+            f"state of {state['shape']} {state['format']} for a layer of {(self.out_features, self.in_features)} {self.format}"
+        self.global_scale, self.input_global_scale = state["global_scale"], state["input_global_scale"]
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, format={self.format!r}, "
+                f"bias={self.bias is not None}, gated={self.gated}")

@@ -111,6 +111,23 @@ def test_python_entry_points_refuse():
             ashqk.quantize_fp4(x)
 
 
+def test_fp4_linear_state_and_refusals():
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8)  # noqa: E731
+    w = lambda fmt="nvfp4", g=0.5: ashqk.FP4Tensor(u8(8, 32), u8(1, 1, 32, 4, 4), (8, 64), fmt, g)  # noqa: E731
+    layer = ashqk.FP4Linear(w(), torch.zeros(8), input_global_scale=0.25)
+    assert (layer.in_features, layer.out_features) == (64, 8) and "nvfp4" in repr(layer)
+    other = ashqk.FP4Linear(w(g=1.0), torch.ones(8))
+    other.load_state_dict(layer.state_dict())
+    assert other.global_scale == 0.5 and other.input_global_scale == 0.25 and float(other.bias.sum()) == 0
+    assert other.weight.shape == (8, 64) and other.weight.global_scale == 0.5
+    with pytest.raises(AssertionError):
+        ashqk.FP4Linear(w(), torch.zeros(7))
+    with pytest.raises(AssertionError):
+        ashqk.FP4Linear(w("mxfp4", 1.0), input_global_scale=0.5)
+    with pytest.raises(AssertionError):
+        ashqk.FP4Linear(w("mxfp4", 1.0), torch.zeros(8)).load_state_dict(layer.state_dict())
+
+
 VP, I64, CI, CF = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 FAKE = 0x10000  # never dereferenced: validation fails first
 

@@ -437,6 +437,40 @@ def test_mlp_in_a_graph_on_another_stream(fmt, m):
         assert torch.equal(yg, want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_awq_checkpoint_layers_as_fp4(fmt):
+    """``replace_linear_layers`` with a 4-bit float format: each layer multiplies the AWQ weights, quantised again."""
+    from ashqk.awq_checkpoint import AWQLayer, replace_linear_layers
+    from oracle import awq_oracle as O
+
+    layers, dense = {}, {}
+    for i, (name, n, k) in enumerate((("up", 384, 256), ("down", 256, 384))):
+        _, qw, qz, s = O.make_problem(1, n, k, 128, seed=i)
+        bias = torch.randn(n, dtype=torch.float16, device="cuda") if name == "down" else None
+        layers[name] = AWQLayer(*(torch.from_numpy(t).cuda() for t in (qw, qz, s)), bias)
+        dense[name] = O.dequantize_awq(qw, qz, s, np.float16).T.astype(np.float64)
+    model = torch.nn.Sequential()
+    model.add_module("up", torch.nn.Linear(256, 384, bias=False))
+    model.add_module("down", torch.nn.Linear(384, 256))
+    assert replace_linear_layers(model, layers, fmt) == ["up", "down"]
+    x = rows(6, 256, "fp16", 1, spread=False)
+    for name in ("up", "down"):
+        layer, w = getattr(model, name), dense[name]
+        g = float(np.float32(np.abs(w).max() / 2688)) if fmt == "nvfp4" else 1.0
+        assert isinstance(layer, ashqk.FP4Linear) and layer.global_scale == g
+        check_quantised(layer.weight, w, fmt, g, *w.shape)
+        code, byte = F.quantize(x.double().cpu().numpy(), fmt)
+        x64, (wc, wb) = F.values(code, byte, fmt), F.quantize(w, fmt, g)
+        w64 = torch.from_numpy(F.values(wc, wb, fmt, g)).cuda()
+        y = layer(x)
+        if layer.bias is None:
+            check_product(y, torch.from_numpy(x64).cuda(), w64, 2.0**-23)
+        else:  # the bias is added to the rounded product
+            assert torch.equal(y, ashqk.w4a4_linear(x, layer.weight) + layer.bias)
+        x = y
+    torch.testing.assert_close(model(rows(6, 256, "fp16", 1, spread=False)), x, rtol=0, atol=0)
+
+
 def test_rows_behind_the_output_are_left_alone():
     """The C ABI writes y's M x N values and nothing else: rows behind and columns beside keep what they held."""
     import ctypes
