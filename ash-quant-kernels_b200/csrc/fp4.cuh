@@ -22,6 +22,8 @@
 
 namespace ashqk {
 
+constexpr int kFp4MaxK = 1 << 24;        // columns; offsets within 128 rows of codes stay below 2^31
+constexpr int64_t kFp4MaxLd = 1 << 24;   // bytes from row to row of codes
 constexpr int kFp4TileRows = 128;
 constexpr int kFp4TileBytes = 512;
 

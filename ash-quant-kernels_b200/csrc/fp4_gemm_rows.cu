@@ -201,8 +201,9 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   if (C > 1) cluster_arrive();
   if (warp == 0 && elect_one()) {
     prefetch_tensormap(&maps.w);
-    for (int kb = kb0; kb < kb1; ++kb) l2_prefetch_2d(&maps.w, kb * 128, n0);
-    const int t0 = kb0 * L::kT, t1 = min(kb1 * L::kT, a.scale_tiles);
+    const int last = min(kb1, kb0 + 32);
+    for (int kb = kb0; kb < last; ++kb) l2_prefetch_2d(&maps.w, kb * 128, n0);
+    const int t0 = kb0 * L::kT, t1 = min(last * L::kT, a.scale_tiles);
     l2_prefetch(a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, (t1 - t0) * kFp4TileBytes);
     if (!FUSED) prefetch_tensormap(&maps.x);
   }

@@ -53,7 +53,7 @@ extern "C" int ashqk_set_fp4_kernel(int which) {
 extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
                                 const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format,
                                 float alpha, void* stream) {
-  if (!y || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || y_ld < N || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!y || M <= 0 || N <= 0 || K <= 0 || K > kFp4MaxK || y_ld < N || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(a_codes, a_ld, a_scales, K)) return rc;
   if (const int rc = check_fp4_operand(b_codes, b_ld, b_scales, K)) return rc;
@@ -64,7 +64,7 @@ extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a
 }
 
 extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes) {
-  if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   size_t offset;
   *bytes = 0;
   if (!fp4_fused_ok(M, N, K)) workspace_layout(M, K, format, &offset, bytes);
@@ -74,7 +74,7 @@ extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t
 extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gated, float x_scale, const void* w_codes,
                                  int64_t w_ld, const void* w_scales, float w_scale, void* y, int64_t y_ld, int M, int N,
                                  int K, int format, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!x || !y || M <= 0 || N <= 0 || K <= 0 || K > (1 << 30) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!x || !y || M <= 0 || N <= 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(x, 2) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (x_ld < static_cast<int64_t>(K) * (gated ? 2 : 1) || y_ld < N) return ASHQK_ERR_INVALID_ARGUMENT;
   if (!fp4_global_scale_ok(format, x_scale) || !fp4_global_scale_ok(format, w_scale)) return ASHQK_ERR_INVALID_ARGUMENT;

@@ -318,6 +318,7 @@ int dtype_size(int dtype) { return dtype == ASHQK_F32 ? 4 : (dtype == ASHQK_F16 
 int check_fp4_operand(const void* codes, int64_t codes_ld, const void* scales, int K) {
   if (!codes || !scales || !aligned(codes, 16) || !aligned(scales, 16)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (codes_ld % 16 || codes_ld < fp4_padded_k(K) / 2) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (codes_ld > kFp4MaxLd) return ASHQK_ERR_UNSUPPORTED;
   return ASHQK_OK;
 }
 
@@ -347,7 +348,7 @@ int quantize_fp4(const void* x, int64_t x_ld, int dtype, bool gated, void* codes
 using namespace ashqk;
 
 extern "C" int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int64_t* scales_bytes) {
-  if (M < 0 || K <= 0 || !fp4_format_ok(format) || !codes_ld || !scales_bytes) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (M < 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format) || !codes_ld || !scales_bytes) return ASHQK_ERR_INVALID_ARGUMENT;
   *codes_ld = fp4_padded_k(K) / 2;
   *scales_bytes = ceil_div64(M, kFp4TileRows) * fp4_scale_tiles(K, format) * kFp4TileBytes;
   return ASHQK_OK;
@@ -356,7 +357,7 @@ extern "C" int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int6
 extern "C" int ashqk_quantize_fp4(const void* x, int64_t x_ld, int dtype, int gated, void* codes, int64_t codes_ld,
                                   void* scales, int M, int K, int format, float global_scale, void* stream) {
   const int size = dtype_size(dtype);
-  if (!x || M <= 0 || K <= 0 || K > (1 << 30) || !size || !aligned(x, size) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!x || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(x, size) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (x_ld < static_cast<int64_t>(K) * (gated ? 2 : 1) || !fp4_global_scale_ok(format, global_scale))
     return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(codes, codes_ld, scales, K)) return rc;
@@ -367,7 +368,7 @@ extern "C" int ashqk_quantize_fp4(const void* x, int64_t x_ld, int dtype, int ga
 extern "C" int ashqk_dequantize_fp4(const void* codes, int64_t codes_ld, const void* scales, void* out, int64_t out_ld,
                                     int dtype, int M, int K, int format, float global_scale, void* stream) {
   const int size = dtype_size(dtype);
-  if (!out || M <= 0 || K <= 0 || K > (1 << 30) || !size || !aligned(out, size) || !fp4_format_ok(format) || out_ld < K ||
+  if (!out || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(out, size) || !fp4_format_ok(format) || out_ld < K ||
       !fp4_global_scale_ok(format, global_scale))
     return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(codes, codes_ld, scales, K)) return rc;

@@ -206,7 +206,7 @@ void check_no_grad(const at::Tensor& x, const char* what) {
 }
 
 void check_fp4(const at::Tensor& codes, const at::Tensor& scales, int64_t K, int64_t format, const at::Device& dev) {
-  TORCH_CHECK(K > 0 && K <= (1 << 30), "ashqk: K out of range");
+  TORCH_CHECK(K > 0 && K <= (1 << 24), "ashqk: K out of range");
   TORCH_CHECK(codes.device() == dev && scales.device() == dev, "ashqk: all tensors must be on the same device");
   TORCH_CHECK(codes.scalar_type() == at::kByte && codes.dim() == 2 && codes.size(1) == (K + 31) / 32 * 16 &&
                   codes.stride(1) == 1,
@@ -233,7 +233,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_fp4(const at::Tensor& x, int64_t for
   check_no_grad(x, "quantize_fp4");
   TORCH_CHECK(format == ASHQK_MXFP4 || format == ASHQK_NVFP4, "ashqk: unknown 4-bit format ", format);
   const int64_t cols = x.size(-1), K = gated ? cols / 2 : cols;
-  TORCH_CHECK(K > 0 && K <= (1 << 30) && (!gated || cols % 2 == 0), "ashqk: x needs columns (an even number when gated)");
+  TORCH_CHECK(K > 0 && K <= (1 << 24) && (!gated || cols % 2 == 0), "ashqk: x needs columns (an even number when gated)");
   c10::cuda::CUDAGuard guard(x.device());
   const Rows r = as_rows(x, cols);
   at::Tensor codes = at::empty({r.rows, (K + 31) / 32 * 16}, x.options().dtype(at::kByte));

@@ -333,7 +333,7 @@ ASHQK_API int ashqk_w4a16_gemv_allreduce(const void* x, int64_t x_ld, const int3
  *                            = Kp / block size; contiguous; padding blocks hold 0, padding rows anything
  *
  * ashqk_fp4_sizes gives the smallest codes_ld and the bytes of scales. codes and scales are 16-byte
- * aligned. For ASHQK_MXFP4 the global scale has to be 1.
+ * aligned; K and codes_ld are at most 2^24. For ASHQK_MXFP4 the global scale has to be 1.
  */
 typedef enum ashqk_fp4_format { ASHQK_MXFP4 = 0, ASHQK_NVFP4 = 1 } ashqk_fp4_format;
 typedef enum ashqk_dtype { ASHQK_F16 = 0, ASHQK_BF16 = 1, ASHQK_F32 = 2 } ashqk_dtype;

@@ -150,7 +150,7 @@ def test_c_abi_sizes():
                             (128, 4096, 1, (2048, 64 * 512)), (0, 64, 1, (32, 0)), (1, 48, 1, (32, 512)), (1, 1, 1, (16, 512))):
         assert lib.ashqk_fp4_sizes(m, k, fmt, ctypes.byref(ld), ctypes.byref(n)) == 0
         assert (ld.value, n.value) == want, (m, k, fmt)
-    for m, k, fmt in ((-1, 32, 0), (1, 0, 0), (1, 32, 2), (1, 32, -1)):
+    for m, k, fmt in ((-1, 32, 0), (1, 0, 0), (1, 32, 2), (1, 32, -1), (1, (1 << 24) + 1, 0)):
         assert lib.ashqk_fp4_sizes(m, k, fmt, ctypes.byref(ld), ctypes.byref(n)) == 1
     size = ctypes.c_size_t()
     for m, n_, k, fmt in ((0, 8, 32, 0), (1, 0, 32, 0), (1, 8, 0, 0), (1, 8, 32, 7)):
@@ -178,7 +178,7 @@ def test_c_abi_refuses_before_the_device():
     quant = dict(x=FAKE, x_ld=64, dtype=0, gated=0, codes=FAKE, codes_ld=32, scales=FAKE, M=2, K=64, format=0, g=1.0, stream=None)
     for args, why in _refusals(quant, [{"x": None}, {"x": FAKE + 1}, {"x_ld": 63}, {"dtype": 3}, {"dtype": -1}, {"gated": 1}, {"codes": None},
                                        {"codes": FAKE + 8}, {"codes_ld": 16}, {"codes_ld": 40}, {"scales": None}, {"scales": FAKE + 4},
-                                       {"M": 0}, {"M": -1}, {"K": 0}, {"format": 2}, {"g": 2.0}, {"format": 1, "g": 0.0},
+                                       {"M": 0}, {"M": -1}, {"K": 0}, {"K": 1 << 25, "x_ld": 1 << 25, "codes_ld": 1 << 24}, {"format": 2}, {"g": 2.0}, {"format": 1, "g": 0.0},
                                        {"format": 1, "g": float("nan")}, {"dtype": 2, "x": FAKE + 2}]):
         assert lib.ashqk_quantize_fp4(*args) == 1, why
     dequant = dict(codes=FAKE, codes_ld=32, scales=FAKE, out=FAKE, out_ld=64, dtype=0, M=2, K=64, format=0, g=1.0, stream=None)
@@ -194,5 +194,7 @@ def test_c_abi_refuses_before_the_device():
     for args, why in _refusals(lin, [{"x": None}, {"x_ld": 32}, {"dtype": 2}, {"gated": 1}, {"xg": 0.5}, {"w": None}, {"w_ld": 8}, {"ws": None},
                                      {"wg": 3.0}, {"y": None}, {"y_ld": 4}, {"M": 0}, {"N": -2}, {"K": 0}, {"format": 3}]):
         assert lib.ashqk_w4a4_linear(*args) == 1, why
+    assert lib.ashqk_quantize_fp4(*{**quant, "codes_ld": (1 << 24) + 16}.values()) == 2  # rows too far apart
+    assert lib.ashqk_fp4_matmul(*{**mm, "b_ld": 1 << 25}.values()) == 2
     for change in ({"work": None}, {"bytes": 100}, {"work": FAKE + 8}):
         assert lib.ashqk_w4a4_linear(*{**lin, **change}.values()) == 3, change

@@ -278,6 +278,39 @@ def test_matmul_nan_stays_in_its_row_and_column(fmt, m):
     assert torch.equal(torch.isnan(y), want)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m", [3, 30, 200])
+def test_linear_nan_and_infinity_stay_in_their_rows(fmt, gated, m):
+    x = rows(m, 512 if gated else 256, "bf16", 5, spread=False)
+    x[1, 100], x[2, 255] = float("nan"), float("inf")
+    w, _ = random_operand(140, 256, fmt, 1)
+    y = ashqk.w4a4_linear(x, w, gated=gated)
+    want = torch.zeros(m, 140, dtype=torch.bool, device="cuda")
+    want[1], want[2] = True, True
+    assert torch.equal(torch.isnan(y), want)
+
+
+def test_long_rows_and_far_apart_codes():
+    """A row of a million columns, and codes whose rows lie megabytes apart."""
+    k = (1 << 20) + 96
+    x = rows(2, k, "bf16", 1, spread=False)
+    for fmt in FORMATS:
+        check_quantised(ashqk.quantize_fp4(x, fmt), x.double().cpu().numpy(), fmt, 1.0, 2, k)
+        w, w64 = random_operand(3, k, fmt, 2)
+        a, a64 = random_operand(2, k, fmt, 3)
+        check_product(ashqk.fp4_matmul(a, w, torch.bfloat16), a64, w64)
+        q = ashqk.quantize_fp4(x, fmt)
+        v64 = ashqk.dequantize_fp4(q).double()
+        check_product(ashqk.w4a4_linear(x, w), v64, w64)
+        wide = torch.zeros(130, 1 << 22, dtype=torch.uint8, device="cuda")
+        b, b64 = random_operand(130, 512, fmt, 4)
+        wide[:, :256] = b.codes
+        far = ashqk.FP4Tensor(wide[:, :256], b.scales, b.shape, fmt)
+        assert torch.equal(ashqk.dequantize_fp4(far), ashqk.dequantize_fp4(b))
+        check_product(ashqk.fp4_matmul(far, b, torch.bfloat16), b64, b64)
+
+
 LINEAR = [(1, 6144, 4096), (1, 100, 64), (2, 4096, 12288), (4, 129, 96), (8, 1024, 1000), (13, 256, 4103), (16, 512, 2048), (17, 128, 4096), (31, 300, 320),
           (64, 256, 512), (130, 384, 1024), (300, 640, 800)]
 
