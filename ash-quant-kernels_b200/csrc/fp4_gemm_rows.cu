@@ -16,8 +16,8 @@
 //               -> the shared memory of the CTA that adds these rows of A, counted in bytes on its barrier
 //               (st.async, or with 32 columns and more through own shared memory and bulk copies)
 //
-// The scales' TMEM columns are double-buffered: stage i's copies wait for the MMAs of stage i - 2. All
-// waits are bounded.
+// The scales have two to eight buffers in TMEM: the copies of stage i wait for the MMAs of stage i - buffers. With
+// two, that wait and not the tensor core set the pace of narrow tiles. All waits are bounded.
 #include <algorithm>
 #include <atomic>
 
@@ -67,12 +67,12 @@ struct RowsShape {
   // Fused: the quantised slice, [stage][row][128] and after it the scale tiles, of which only the first NT rows
   // are there: the copy to TMEM reads on into the next tile, for rows that nobody uses.
   static constexpr uint32_t kXSTile = NT * 16;
-  // TMEM: the sums, then two buffers of scales.
+  // TMEM: the sums, then as many buffers of scales as fit.
   static constexpr int kSfW = kT * 4, kSfX = kT * 4;
   static constexpr int kSf0 = NT < 32 ? 32 : NT;
-  static constexpr int kCols = kSf0 + 2 * (kSfW + kSfX);
-  static constexpr uint32_t kTmemCols = kCols <= 64 ? 64 : kCols <= 128 ? 128 : 256;
-  static_assert(kCols <= 256, "TMEM");
+  static constexpr uint32_t kTmemCols = NT <= 64 ? 128 : 256;
+  static constexpr int kSfBufs = (static_cast<int>(kTmemCols) - kSf0) / (kSfW + kSfX);
+  static_assert(kSfBufs >= 2, "TMEM");
   // Split K: whether the slots for partial sums have shared memory of their own or take the ring's, and whether
   // the sums go there by way of the own ring.
   static constexpr bool kOwnSlots = NT <= 32;
@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
       mbar_drain(&full[f % a.ring], static_cast<uint32_t>(f / a.ring) & 1u);
     }
   } else if (warp == 1) {
-    int stage = 0, old = 0;  // stage of kb, of kb - 2
+    int stage = 0, old = 0, buf = 0;  // stage of kb, of kb - kSfBufs; scale buffer
     uint32_t phase = 0, old_phase = 0;
     bool ok = !FUSED || mbar_wait(x_ready, 0, abort, true);
     for (int kb = kb0; ok && kb < kb1; ++kb) {
@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         ok = false;
         break;
       }
-      if (i >= 2) {
+      // (In a ring of no more stages than buffers the wait above has seen to it: the producer waited for stage i - ring.)
+      if (L::kSfBufs < a.ring && i >= L::kSfBufs) {
         if (!mbar_wait(&empty[old], old_phase, abort, true)) {
           ok = false;
           break;
@@ -275,7 +276,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
       }
       tc_fence_after_sync();
       const uint32_t base = sbase + stage * L::kStage;
-      const uint32_t sfw = tmem + L::kSf0 + (i & 1) * (L::kSfW + L::kSfX);
+      const uint32_t sfw = tmem + L::kSf0 + buf * (L::kSfW + L::kSfX);
+      if (++buf == L::kSfBufs) buf = 0;
       const uint32_t sfx = sfw + L::kSfW;
       const uint64_t sd = scale_tile_desc(base + L::kW);
       const uint64_t sx = scale_tile_desc(FUSED ? x_scales + i * L::kT * L::kXSTile : base + L::kW + L::kWS + L::kX);
@@ -441,7 +443,6 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
 
 std::atomic<int> g_cluster{0}, g_ring{0};
 
-// At least two stages: the wait for stage i - 2 counts on the producer not having passed it twice.
 struct RowsPlan {
   int cluster, ring;
   uint32_t off_x, off_slots, off_bar, smem;
