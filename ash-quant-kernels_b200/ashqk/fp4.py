@@ -42,9 +42,12 @@ def _format(fmt: str) -> int:
     return code
 
 
-def _check_global_scale(fmt: str, g: float) -> None:
-    assert g == 1.0 if fmt == "mxfp4" else 1e-18 <= g <= 1e18, \
+def _check(fmt: str, g: float) -> int:
+    """The format's code, after checking it and a global scale for it."""
+    code = _format(fmt)
+    assert (1e-18 <= g <= 1e18) if code else g == 1.0, \
         f"global_scale {g} out of range (1 for mxfp4, 1e-18 .. 1e18 for nvfp4)"
+    return code
 
 
 class FP4Tensor:
@@ -68,8 +71,7 @@ class FP4Tensor:
     def from_rowmajor(codes: torch.Tensor, scales: torch.Tensor, format: str = "mxfp4", global_scale: float = 1.0) -> "FP4Tensor":
         """From a checkpoint's plain layout: codes uint8 [rows, K / 2], scales [rows, K / block] (uint8, or float8
         of the format's kind). K is a multiple of the block."""
-        _format(format)
-        _check_global_scale(format, global_scale)
+        _check(format, global_scale)
         block = _BLOCK[format]
         assert codes.dtype == torch.uint8 and codes.dim() == 2 and scales.dim() == 2
         rows, k = codes.shape[0], 2 * codes.shape[1]
@@ -110,24 +112,14 @@ def fp4_global_scale(x: torch.Tensor) -> float:
     return g if g >= 1e-18 else 1.0
 
 
-def _quantize(x: torch.Tensor, fmt: str, global_scale: float, gated: bool) -> FP4Tensor:
-    code = _format(fmt)
-    _check_global_scale(fmt, global_scale)
-    k = x.shape[-1]
-    if gated:
-        assert k % 2 == 0, "gate and up are the two halves of the last dimension"
-        k //= 2
-    codes, scales = _op("quantize_fp4")(x, code, global_scale, gated)
-    return FP4Tensor(codes, scales, (codes.shape[0], k), fmt, global_scale)
-
-
 def quantize_fp4(x: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
     """x [..., K] (fp16, bf16 or fp32) -> FP4Tensor of shape (rows, K); any K, strided rows as they are.
 
     ``global_scale`` belongs to "nvfp4" (see ``fp4_global_scale``); a block with an infinity or a NaN
     reads back as NaN.
     """
-    return _quantize(x, format, global_scale, False)
+    codes, scales = _op("quantize_fp4")(x, _check(format, global_scale), global_scale, False)
+    return FP4Tensor(codes, scales, (codes.shape[0], x.shape[-1]), format, global_scale)
 
 
 def silu_mul_quantize_fp4(gate_up: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
@@ -135,7 +127,10 @@ def silu_mul_quantize_fp4(gate_up: torch.Tensor, format: str = "mxfp4", *, globa
 
     The activation is computed in fp32 and rounded once, to the format: one pass over gate_up.
     """
-    return _quantize(gate_up, format, global_scale, True)
+    k = gate_up.shape[-1]
+    assert k % 2 == 0, "gate and up are the two halves of the last dimension"
+    codes, scales = _op("quantize_fp4")(gate_up, _check(format, global_scale), global_scale, True)
+    return FP4Tensor(codes, scales, (codes.shape[0], k // 2), format, global_scale)
 
 
 def dequantize_fp4(q: FP4Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -158,9 +153,8 @@ def w4a4_linear(x: torch.Tensor, weight: FP4Tensor, *, global_scale: float = 1.0
     ``gated``: x is [..., 2 K] and silu(x[..., :K]) * x[..., K:] takes its place (an MLP's down
     projection). ``global_scale`` is x's, for "nvfp4".
     """
-    _check_global_scale(weight.format, global_scale)
-    return _op("w4a4_linear")(x, weight.codes, weight.scales, weight.shape[1], _format(weight.format), global_scale,
-                              weight.global_scale, gated)
+    return _op("w4a4_linear")(x, weight.codes, weight.scales, weight.shape[1], _check(weight.format, global_scale),
+                              global_scale, weight.global_scale, gated)
 
 
 class FP4Linear(torch.nn.Module):
@@ -171,7 +165,7 @@ class FP4Linear(torch.nn.Module):
 
     def __init__(self, weight: FP4Tensor, bias: torch.Tensor | None = None, *, input_global_scale: float = 1.0, gated: bool = False):
         super().__init__()
-        _check_global_scale(weight.format, input_global_scale)
+        _check(weight.format, input_global_scale)
         assert bias is None or bias.shape == (weight.shape[0],), f"bias {tuple(bias.shape)} for {weight.shape[0]} outputs"
         self.register_buffer("codes", weight.codes)
         self.register_buffer("scales", weight.scales)
