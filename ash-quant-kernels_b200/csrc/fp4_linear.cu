@@ -26,6 +26,7 @@ int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_
 namespace {
 
 std::atomic<int> g_matmul_kernel{0};
+constexpr int kMaxRows = 1 << 30;  // of either operand: tile coordinates are 32-bit
 
 // Few rows go to the rows kernel, whose CTAs split K, the others to CTA pairs. Measured in graphs (MXFP4, us, rows
 // against pairs): 64 rows 8.2 / 9.4 (4096->6144), 7.9 / 9.1 (4096->4096), 10.9 / 14.9 (12288->4096), 15.2 / 17.6
@@ -55,6 +56,7 @@ extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a
                                 float alpha, void* stream) {
   if (!y || M <= 0 || N <= 0 || K <= 0 || K > kFp4MaxK || y_ld < N || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (M > kMaxRows || N > kMaxRows) return ASHQK_ERR_UNSUPPORTED;
   if (const int rc = check_fp4_operand(a_codes, a_ld, a_scales, K)) return rc;
   if (const int rc = check_fp4_operand(b_codes, b_ld, b_scales, K)) return rc;
   const int which = g_matmul_kernel.load(std::memory_order_relaxed);
@@ -78,6 +80,7 @@ extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gat
   if ((dtype != ASHQK_F16 && dtype != ASHQK_BF16) || !aligned(x, 2) || !aligned(y, 2)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (x_ld < static_cast<int64_t>(K) * (gated ? 2 : 1) || y_ld < N) return ASHQK_ERR_INVALID_ARGUMENT;
   if (!fp4_global_scale_ok(format, x_scale) || !fp4_global_scale_ok(format, w_scale)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (M > kMaxRows || N > kMaxRows) return ASHQK_ERR_UNSUPPORTED;
   if (const int rc = check_fp4_operand(w_codes, w_ld, w_scales, K)) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fp4_fused_ok(M, N, K))

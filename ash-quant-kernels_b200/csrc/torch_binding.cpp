@@ -196,7 +196,7 @@ Rows as_rows(const at::Tensor& x, int64_t cols) {
   r.t = x.dim() == 2 ? x : x.reshape({cols ? x.numel() / cols : 0, cols});
   if (r.t.stride(1) != 1 || (r.t.size(0) > 1 && r.t.stride(0) < cols)) r.t = r.t.contiguous();
   r.rows = r.t.size(0);
-  r.ld = r.rows > 1 ? r.t.stride(0) : cols;
+  r.ld = r.rows > 1 ? r.t.stride(0) : (cols + 31) / 32 * 32;  // of one row only its start's alignment counts
   TORCH_CHECK(r.rows <= INT32_MAX, "ashqk: problem too large");
   return r;
 }

@@ -352,8 +352,9 @@ ASHQK_API int ashqk_dequantize_fp4(const void* codes, int64_t codes_ld, const vo
                                    int dtype, int M, int K, int format, float global_scale, void* stream);
 
 /*
- * y [M, N] (ashqk_dtype F16 or BF16, row stride y_ld elements) = alpha * A @ B^T for quantised A [M, K] and
- * B [N, K] of one format; alpha carries the global scales' product. fp32 accumulation.
+ * y [M, N] (ashqk_dtype F16 or BF16, row stride y_ld elements, any alignment of a value) = alpha * A @ B^T for
+ * quantised A [M, K] and B [N, K] of one format; alpha carries the global scales' product. fp32 accumulation.
+ * M and N up to 2^30.
  */
 ASHQK_API int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes,
                                int64_t b_ld, const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K,

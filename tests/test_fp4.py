@@ -196,5 +196,7 @@ def test_c_abi_refuses_before_the_device():
         assert lib.ashqk_w4a4_linear(*args) == 1, why
     assert lib.ashqk_quantize_fp4(*{**quant, "codes_ld": (1 << 24) + 16}.values()) == 2  # rows too far apart
     assert lib.ashqk_fp4_matmul(*{**mm, "b_ld": 1 << 25}.values()) == 2
+    assert lib.ashqk_fp4_matmul(*{**mm, "M": (1 << 30) + 1}.values()) == 2
+    assert lib.ashqk_w4a4_linear(*{**lin, "N": (1 << 30) + 1, "y_ld": 1 << 31}.values()) == 2
     for change in ({"work": None}, {"bytes": 100}, {"work": FAKE + 8}):
         assert lib.ashqk_w4a4_linear(*{**lin, **change}.values()) == 3, change

@@ -471,6 +471,61 @@ def test_mlp_in_a_graph_on_another_stream(fmt, m):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [1, 20, 40, 300])
+def test_weights_and_inputs_written_right_before_their_use(fmt, m):
+    """No wait between writing weights, writing x and multiplying: the product sees both as written."""
+    stage = [rows(512, 1024, "bf16", s, spread=False) for s in range(4)]
+    xs = [rows(m, 1024, "bf16", 10 + s, spread=False) for s in range(4)]
+    w, x = torch.empty_like(stage[0]), torch.empty_like(xs[0])
+    q = ashqk.quantize_fp4(stage[0], fmt, global_scale=G[fmt])
+    codes, scales = torch.empty_like(q.codes), torch.empty_like(q.scales)
+    held = ashqk.FP4Tensor(codes, scales, q.shape, fmt, G[fmt])
+    got = []
+    for i in range(24):
+        w.copy_(stage[i % 4])
+        x.copy_(xs[i % 3])
+        if i % 2:  # codes rewritten in place by a copy, or a new tensor straight from the quantiser
+            new = ashqk.quantize_fp4(w, fmt, global_scale=G[fmt])
+            codes.copy_(new.codes)
+            scales.copy_(new.scales)
+            got.append(ashqk.w4a4_linear(x, held, global_scale=G[fmt]))
+        else:
+            got.append(ashqk.w4a4_linear(x, ashqk.quantize_fp4(w, fmt, global_scale=G[fmt]), global_scale=G[fmt]))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        qw = ashqk.quantize_fp4(stage[i % 4], fmt, global_scale=G[fmt])
+        torch.cuda.synchronize()
+        assert torch.equal(y, ashqk.w4a4_linear(xs[i % 3], qw, global_scale=G[fmt])), i
+
+
+def test_calls_on_several_streams_at_once():
+    """Products of both kernels, quantisers and an AWQ layer side by side on four streams: each gives what it gives alone."""
+    from oracle import awq_oracle as O
+
+    jobs = []
+    for i, (m, n, k, fmt) in enumerate(((1, 4096, 4096, "nvfp4"), (16, 2048, 4096, "mxfp4"), (50, 1024, 8192, "nvfp4"), (100, 1536, 2048, "mxfp4"),
+                                        (300, 1024, 8192, "mxfp4"), (700, 2048, 1024, "nvfp4"))):
+        w, _ = random_operand(n, k, fmt, i)
+        x = rows(m, k, "fp16", i, spread=False)
+        jobs.append(lambda x=x, w=w: ashqk.w4a4_linear(x, w))
+    xa, qw, qz, s = (torch.from_numpy(t).cuda() for t in O.make_problem(4, 4096, 2048, 128, seed=3))
+    jobs.append(lambda: ashqk.w4a16_linear(xa, qw, qz, s))
+    xb = xa.repeat(64, 1)
+    jobs.append(lambda: ashqk.w4a16_linear(xb, qw, qz, s))
+    want = [j() for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = []
+    for r in range(12):
+        for i, j in enumerate(jobs):
+            with torch.cuda.stream(streams[(i + r) % 4]):
+                got.append((i, j()))
+    torch.cuda.synchronize()
+    for i, y in got:
+        assert torch.equal(y, want[i]), i
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_awq_checkpoint_layers_as_fp4(fmt):
     """``replace_linear_layers`` with a 4-bit float format: each layer multiplies the AWQ weights, quantised again."""
     from ashqk.awq_checkpoint import AWQLayer, replace_linear_layers
