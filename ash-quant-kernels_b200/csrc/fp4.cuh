@@ -34,9 +34,52 @@ __host__ __device__ constexpr int64_t fp4_padded_k(int64_t k) { return (k + 31) 
 __host__ __device__ constexpr int64_t fp4_scale_tiles(int64_t k, int format) {
   return (fp4_padded_k(k) / fp4_block(format) + 3) / 4;
 }
-__device__ __forceinline__ int64_t fp4_scale_offset(int64_t row, int block, int64_t tiles) {
+// Offset of the scale of (row, block); I: 32 or 64 bits.
+template <typename I>
+__device__ __forceinline__ I fp4_scale_offset(I row, uint32_t block, I tiles) {
   return ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
+
+// ---- the host functions that the files share ----------------------------------------------------
+
+// A quantised matrix of `rows` rows.
+struct Fp4Matrix {
+  const uint8_t* codes;
+  int64_t ld;
+  const uint8_t* scales;
+  int rows;
+};
+// y [a.rows, b.rows] = alpha * a b^T; dtype F16 or BF16.
+struct Fp4Product {
+  Fp4Matrix a, b;
+  int K, format;
+  float alpha;
+  void* y;
+  int64_t y_ld;
+  int dtype;
+};
+// What is to be quantised: 16- or 32-bit rows, gated or not.
+struct Fp4Source {
+  const void* x;
+  int64_t ld;
+  int dtype;
+  bool gated;
+  float gs;
+};
+
+int dtype_size(int dtype);  // 0: no such type
+int check_fp4_operand(const void* codes, int64_t codes_ld, const void* scales, int K);
+bool fp4_global_scale_ok(int format, float gs);
+// `early`: let the next launch start while this one runs. Only for a consumer that reads the result
+// behind its own griddepcontrol.wait.
+int quantize_fp4(const Fp4Source& x, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, int format, bool early,
+                 cudaStream_t stream);
+int fp4_matmul_rows(const Fp4Product& p, cudaStream_t stream);
+int fp4_matmul_pair(const Fp4Product& p, cudaStream_t stream);
+bool fp4_fused_ok(int M, int N, int K);
+// p.a is not used but for its rows.
+int fp4_linear_rows(const Fp4Source& x, const Fp4Product& p, cudaStream_t stream);
+void fp4_set_pair_split(int split);
 
 // What a quantiser needs of the global scale g; on the host.
 struct Fp4Quant {
@@ -263,8 +306,8 @@ __device__ __forceinline__ void load16(const T* p, int count, int align, Raw16<T
 #pragma unroll
     for (int i = 0; i < kWords; i += 8)
       asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]), "=r"(r.w[i + 5]),
-                     "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
+                   : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3]), "=r"(r.w[i + 4]),
+                     "=r"(r.w[i + 5]), "=r"(r.w[i + 6]), "=r"(r.w[i + 7])
                    : "l"(reinterpret_cast<const uint32_t*>(p) + i)
                    : "memory");
   } else if (align == 16) {

@@ -87,8 +87,8 @@ __device__ __forceinline__ void tile_of(const PairArgs& a, int t, int& tm, int& 
 // TMA load completing on the barrier (cluster address) of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          smem_u32(dst)),
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
@@ -101,7 +101,8 @@ __device__ __forceinline__ uint16_t lds_u16(uint32_t addr) {
 
 // 64 fp32 columns of one row, times alpha, as 16-bit pairs.
 template <typename T>
-__device__ __forceinline__ void round_row64(const uint32_t (&r0)[32], const uint32_t (&r1)[32], float alpha, uint32_t (&h)[32]) {
+__device__ __forceinline__ void round_row64(const uint32_t (&r0)[32], const uint32_t (&r1)[32], float alpha,
+                                            uint32_t (&h)[32]) {
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     h[i] = pack2<T>(alpha * __uint_as_float(r0[2 * i]), alpha * __uint_as_float(r0[2 * i + 1]));
@@ -110,8 +111,8 @@ __device__ __forceinline__ void round_row64(const uint32_t (&r0)[32], const uint
 }
 
 // An epilogue warp's 32 rows x 64 columns of sums -> y. `out`: its staging buffer.
-__device__ __forceinline__ void store_tile(const PairMaps& maps, const PairArgs& a, const uint32_t (&r0)[32], const uint32_t (&r1)[32],
-                                           unsigned char* out, int row0, int n, int lane) {
+__device__ __forceinline__ void store_tile(const PairMaps& maps, const PairArgs& a, const uint32_t (&r0)[32],
+                                           const uint32_t (&r1)[32], unsigned char* out, int row0, int n, int lane) {
   uint32_t v[32];
   if (a.bf16)
     round_row64<__nv_bfloat16>(r0, r1, a.alpha, v);
@@ -386,8 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1) fp4_pair_kernel(const __grid_cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[i] = __float_as_uint(__uint_as_float(p[i]) + __uint_as_float(w[i]));
         }
-        store_tile(maps, a, r[0], r[1], smem + L::off_out + (warp - kFirstEpiWarp) * L::kOut,
-                   tm * (2 * kBM) + static_cast<int>(rank) * kBM + 32 * quad, tn * kBN + 128 * part_k + 64 * part, lane);
+        const int row0 = tm * (2 * kBM) + static_cast<int>(rank) * kBM + 32 * quad;
+        store_tile(maps, a, r[0], r[1], smem + L::off_out + (warp - kFirstEpiWarp) * L::kOut, row0,
+                   tn * kBN + 128 * part_k + 64 * part, lane);
       }
       if (lane == 0) bulk_wait();
     }
@@ -469,43 +471,46 @@ int run_pair(const PairMaps& maps, const PairArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int fp4_matmul_pair(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
-                    const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
-                    cudaStream_t stream) {
+int fp4_matmul_pair(const Fp4Product& p, cudaStream_t stream) {
+  const int M = p.a.rows, N = p.b.rows;
   PairArgs a;
-  a.y = y;
-  a.y_ld = y_ld;
+  a.y = p.y;
+  a.y_ld = p.y_ld;
   a.M = M;
   a.N = N;
-  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(K), 64));
-  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(K), kFp4BlockK));
+  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(p.K), 64));
+  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(p.K), kFp4BlockK));
   a.tiles_m = ceil_div(M, 2 * kBM);
   a.tiles_n = ceil_div(N, kBN);
   if (static_cast<int64_t>(a.tiles_m) * a.tiles_n > (1 << 30)) return ASHQK_ERR_UNSUPPORTED;
-  a.alpha = alpha;
-  a.bf16 = dtype == ASHQK_BF16;
-  a.tma_y = aligned(y, 16) && y_ld % 8 == 0;
-  const uint64_t row_bytes = fp4_padded_k(K) / 2;
-  const uint64_t scale_bytes = fp4_scale_tiles(K, format) * kFp4TileBytes;
-  const uint32_t stage_scales = kFp4BlockK / fp4_block(format) / 4 * kFp4TileBytes;
-  PairMaps maps;
-  int rc = encode_tensor_map_2d(&maps.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(a_codes), row_bytes, M, a_ld, 128,
-                                kBM, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (!rc)
-    rc = encode_tensor_map_2d(&maps.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(b_codes), row_bytes, N, b_ld, 128,
-                              kHalfN, CU_TENSOR_MAP_SWIZZLE_128B);
+  a.alpha = p.alpha;
+  a.bf16 = p.dtype == ASHQK_BF16;
+  a.tma_y = aligned(p.y, 16) && p.y_ld % 8 == 0;
+  const uint64_t row_bytes = fp4_padded_k(p.K) / 2;
+  const uint64_t scale_bytes = fp4_scale_tiles(p.K, p.format) * kFp4TileBytes;
+  const uint32_t stage_scales = kFp4BlockK / fp4_block(p.format) / 4 * kFp4TileBytes;
+  auto codes_map = [&](CUtensorMap* map, const Fp4Matrix& m, int box_rows) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(m.codes), row_bytes, m.rows,
+                                m.ld, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
   // Scale tiles as rows of 8-byte elements: one row per 128 rows of the matrix.
-  if (!rc)
-    rc = encode_tensor_map_2d(&maps.as, CU_TENSOR_MAP_DATA_TYPE_UINT64, const_cast<void*>(a_scales), scale_bytes / 8,
-                              ceil_div(M, kFp4TileRows), scale_bytes, stage_scales / 8, 1, CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (!rc)
-    rc = encode_tensor_map_2d(&maps.bs, CU_TENSOR_MAP_DATA_TYPE_UINT64, const_cast<void*>(b_scales), scale_bytes / 8,
-                              ceil_div(N, kFp4TileRows), scale_bytes, stage_scales / 8, 2, CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (!rc)
-    rc = a.tma_y ? encode_tensor_map_2d(&maps.y, CU_TENSOR_MAP_DATA_TYPE_UINT16, y, N, M, y_ld * 2, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B)
-                 : (maps.y = maps.a, ASHQK_OK);
+  auto scales_map = [&](CUtensorMap* map, const Fp4Matrix& m, int box_rows) {
+    return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, const_cast<uint8_t*>(m.scales), scale_bytes / 8,
+                                ceil_div(m.rows, kFp4TileRows), scale_bytes, stage_scales / 8, box_rows,
+                                CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  PairMaps maps;
+  int rc = codes_map(&maps.a, p.a, kBM);
+  if (!rc) rc = codes_map(&maps.b, p.b, kHalfN);
+  if (!rc) rc = scales_map(&maps.as, p.a, 1);
+  if (!rc) rc = scales_map(&maps.bs, p.b, 2);
+  if (!rc && a.tma_y)
+    rc = encode_tensor_map_2d(&maps.y, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.y, N, M, p.y_ld * 2, 64, 32,
+                              CU_TENSOR_MAP_SWIZZLE_128B);
+  else
+    maps.y = maps.a;  // not used
   if (rc) return rc;
-  return format == ASHQK_MXFP4 ? run_pair<ASHQK_MXFP4>(maps, a, stream) : run_pair<ASHQK_NVFP4>(maps, a, stream);
+  return p.format == ASHQK_MXFP4 ? run_pair<ASHQK_MXFP4>(maps, a, stream) : run_pair<ASHQK_NVFP4>(maps, a, stream);
 }
 
 void fp4_set_pair_split(int split) { g_split.store(split, std::memory_order_relaxed); }

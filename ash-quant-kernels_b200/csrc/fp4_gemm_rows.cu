@@ -24,9 +24,6 @@
 #include "fp4_mma.cuh"
 
 namespace ashqk {
-
-void fp4_set_pair_split(int split);
-
 namespace {
 
 constexpr int kTileN = 128;  // weight rows per CTA
@@ -89,13 +86,15 @@ __device__ __forceinline__ void l2_prefetch_2d(const CUtensorMap* map, int x, in
                : "memory");
 }
 __device__ __forceinline__ void l2_prefetch(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes)
+               : "memory");
 }
 
 // Quantises columns [256 kb0, 256 kb1) of A's rows into shared memory, sixteen columns per thread, as the quantiser
 // proper does.
 template <int FMT, int NT, typename T, bool GATED>
-__device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int kb1, uint32_t codes, uint32_t scales, int tid) {
+__device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int kb1, uint32_t codes, uint32_t scales,
+                                               int tid) {
   using L = RowsShape<FMT, NT, true>;
   constexpr int kLanes = fp4_block(FMT) / 16;
   constexpr int kBatch = GATED ? 1 : 2;  // chunks whose loads are in flight together
@@ -143,7 +142,8 @@ __device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int k
       const uint32_t byte = fp4_quantize16<FMT>(v, amax, a.xq, &c);
       if (i0 + b * kStep < total) {
         const int m = row[b], kb = chunk[b] >> 4, cc = chunk[b] & 15;
-        const uint32_t at = codes + kb * L::kX + (m >> 3) * 1024 + (m & 7) * 128 + (((cc >> 1) ^ (m & 7)) << 4) + (cc & 1) * 8;
+        const uint32_t at =
+            codes + kb * L::kX + (m >> 3) * 1024 + (m & 7) * 128 + (((cc >> 1) ^ (m & 7)) << 4) + (cc & 1) * 8;
         asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c.x), "r"(c.y) : "memory");
         if (cc % kLanes == 0) {
           const int block = cc / kLanes;
@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   const int m0 = static_cast<int>(blockIdx.y) * NT;
   const int kb0 = static_cast<int>(static_cast<int64_t>(a.num_kb) * rank / C);
   const int kb1 = static_cast<int>(static_cast<int64_t>(a.num_kb) * (rank + 1) / C);
+  const uint8_t* ws = a.ws + static_cast<int64_t>(tile) * a.scale_tiles * kFp4TileBytes;
   // Groups of four rows of A; group g's partial sums are added by the CTA of rank g % C.
   const int groups = (min(NT, a.M - m0) + 3) / 4;
   const int my_groups = (groups - rank + C - 1) / C;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
     const int last = min(kb1, kb0 + 32);
     for (int kb = kb0; kb < last; ++kb) l2_prefetch_2d(&maps.w, kb * 128, n0);
     const int t0 = kb0 * L::kT, t1 = min(last * L::kT, a.scale_tiles);
-    l2_prefetch(a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, (t1 - t0) * kFp4TileBytes);
+    l2_prefetch(ws + static_cast<int64_t>(t0) * kFp4TileBytes, (t1 - t0) * kFp4TileBytes);
     if (!FUSED) prefetch_tensormap(&maps.x);
   }
   if (warp == 1) {
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   const uint32_t x_scales = x_codes + static_cast<uint32_t>(kb1 - kb0) * L::kX;
 
   if (warp == 0) {
+    const uint8_t* xs = a.xs + static_cast<int64_t>(m0 / kFp4TileRows) * a.scale_tiles * kFp4TileBytes;
     int stage = 0;
     uint32_t phase = 0;
     int issued = 0;
@@ -235,11 +237,10 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
       if (elect_one()) {
         mbar_arrive_expect_tx(&full[stage], L::kW + sf + (FUSED ? 0 : L::kX + sf));
         tma_load_2d(base, &maps.w, kb * 128, n0, &full[stage]);
-        bulk_load(base + L::kW, a.ws + (static_cast<int64_t>(tile) * a.scale_tiles + t0) * kFp4TileBytes, sf, &full[stage]);
+        bulk_load(base + L::kW, ws + static_cast<int64_t>(t0) * kFp4TileBytes, sf, &full[stage]);
         if (!FUSED) {
           tma_load_2d(base + L::kW + L::kWS, &maps.x, kb * 128, m0, &full[stage]);
-          bulk_load(base + L::kW + L::kWS + L::kX, a.xs + (static_cast<int64_t>(m0 / kFp4TileRows) * a.scale_tiles + t0) * kFp4TileBytes,
-                    sf, &full[stage]);
+          bulk_load(base + L::kW + L::kWS + L::kX, xs + static_cast<int64_t>(t0) * kFp4TileBytes, sf, &full[stage]);
         }
       }
       __syncwarp();
@@ -263,7 +264,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         ok = false;
         break;
       }
-      // (In a ring of no more stages than buffers the wait above has seen to it: the producer waited for stage i - ring.)
+      // (In a ring of no more stages than buffers the wait above has seen to it: the producer waited for stage
+      // i - ring.)
       if (L::kSfBufs < a.ring && i >= L::kSfBufs) {
         if (!mbar_wait(&empty[old], old_phase, abort, true)) {
           ok = false;
@@ -351,8 +353,9 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   auto store4 = [&](int m, float v0, float v1, float v2, float v3) {
     if (n >= a.N) return;
     uint16_t* y = static_cast<uint16_t*>(a.y) + m * a.y_ld + n;
-    const uint32_t lo = a.bf16 ? pack2<__nv_bfloat16>(v0 * a.alpha, v1 * a.alpha) : pack2<__half>(v0 * a.alpha, v1 * a.alpha);
-    const uint32_t hi = a.bf16 ? pack2<__nv_bfloat16>(v2 * a.alpha, v3 * a.alpha) : pack2<__half>(v2 * a.alpha, v3 * a.alpha);
+    v0 *= a.alpha, v1 *= a.alpha, v2 *= a.alpha, v3 *= a.alpha;
+    const uint32_t lo = a.bf16 ? pack2<__nv_bfloat16>(v0, v1) : pack2<__half>(v0, v1);
+    const uint32_t hi = a.bf16 ? pack2<__nv_bfloat16>(v2, v3) : pack2<__half>(v2, v3);
     if (m < a.M) y[0] = static_cast<uint16_t>(lo);
     if (m + 1 < a.M) y[a.y_ld] = static_cast<uint16_t>(lo >> 16);
     if (m + 2 < a.M) y[2 * a.y_ld] = static_cast<uint16_t>(hi);
@@ -411,13 +414,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         constexpr int kPer = 8;  // groups of one TMEM load
         fence_proxy_async_smem();
         __syncwarp();
-        for (int i = lane; i < (groups + kPer - 1) / kPer * kPer; i += 32) {
-          const int g = i, l = g / C, owner = g - l * C;
-          if (g < groups && ((g / kPer) & 1) == turn && owner != rank) {
-            const uint32_t first = static_cast<uint32_t>(row - lane) * 16;
-            bulk_to_cluster(map_rank(slots + static_cast<uint32_t>((l * C + rank) * kTileN) * 16 + first, owner),
-                            sbase + static_cast<uint32_t>(g * kTileN) * 16 + first, 512, map_rank(smem_u32(received), owner));
-          }
+        const uint32_t first = static_cast<uint32_t>(row - lane) * 16;
+        for (int g = lane; g < groups; g += 32) {
+          const int l = g / C, owner = g - l * C;
+          if (((g / kPer) & 1) != turn || owner == rank) continue;
+          const uint32_t to = slots + static_cast<uint32_t>((l * C + rank) * kTileN) * 16 + first;
+          bulk_to_cluster(map_rank(to, owner), sbase + static_cast<uint32_t>(g * kTileN) * 16 + first, 512,
+                          map_rank(smem_u32(received), owner));
         }
         __syncwarp();
       }
@@ -430,8 +433,10 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
 #pragma unroll 4
         for (int c = 0; c < C; ++c) {
           // without slots of its own, this CTA's sums are still where they were staged
-          const uint4 p = lds_v4(!L::kOwnSlots && c == rank ? sbase + static_cast<uint32_t>((l * C + rank) * kTileN + row) * 16 : slot(l, c));
-          s[0] += __uint_as_float(p.x), s[1] += __uint_as_float(p.y), s[2] += __uint_as_float(p.z), s[3] += __uint_as_float(p.w);
+          const bool staged = !L::kOwnSlots && c == rank;
+          const uint4 p = lds_v4(staged ? sbase + static_cast<uint32_t>((l * C + rank) * kTileN + row) * 16 : slot(l, c));
+          s[0] += __uint_as_float(p.x), s[1] += __uint_as_float(p.y);
+          s[2] += __uint_as_float(p.z), s[3] += __uint_as_float(p.w);
         }
         store4(m0 + 4 * (l * C + rank), s[0], s[1], s[2], s[3]);
       }
@@ -477,9 +482,13 @@ RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   const uint32_t fixed = x_bytes + (L::kOwnSlots ? slots : 0);
   p.ring = fixed + 2 * L::kStage > budget ? 2 : static_cast<int>((budget - fixed) / L::kStage);
   p.ring = std::max(2, std::min({kMaxRing, local, p.ring}));
-  if (const int r = g_ring.load(std::memory_order_relaxed)) p.ring = std::max(2, std::min({r, local, static_cast<int>((222 * 1024 - std::min(fixed, 222u * 1024)) / L::kStage)}));
+  if (const int r = g_ring.load(std::memory_order_relaxed)) {
+    constexpr uint32_t kMost = 222 * 1024;
+    p.ring = std::max(2, std::min({r, local, static_cast<int>((kMost - std::min(fixed, kMost)) / L::kStage)}));
+  }
   uint32_t ring = p.ring * L::kStage;
-  if (p.cluster > 1 && L::kStaged) ring = std::max(ring, (L::kStaging + (L::kOwnSlots ? 0 : slots) + 1023) / 1024 * 1024);
+  if (p.cluster > 1 && L::kStaged)
+    ring = std::max(ring, (L::kStaging + (L::kOwnSlots ? 0 : slots) + 1023) / 1024 * 1024);
   p.off_x = ring;
   p.off_slots = (p.off_x + x_bytes + 15) / 16 * 16;
   p.off_bar = (p.off_slots + (L::kOwnSlots ? slots : 0) + 7) / 8 * 8;
@@ -504,7 +513,8 @@ int launch_rows(const RowsMaps& maps, RowsArgs a, cudaStream_t stream) {
   auto kernel = fp4_rows_kernel<FMT, NT, FUSED>;
   static std::atomic<bool> configured[64];  // zero-initialised (static storage)
   if (!configured[dev.device].load(std::memory_order_acquire)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(dev.max_smem_optin)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(dev.max_smem_optin)) != cudaSuccess)
       return ASHQK_ERR_CUDA;
     configured[dev.device].store(true, std::memory_order_release);
   }
@@ -540,40 +550,39 @@ int launch_rows_fmt(const RowsMaps& maps, const RowsArgs& a, int nt, bool fused,
   }
 }
 
-int rows_args(RowsArgs& a, RowsMaps& maps, const void* b_codes, int64_t b_ld, const void* b_scales, void* y, int64_t y_ld,
-              int dtype, int M, int N, int K, int format, float alpha) {
-  a.ws = static_cast<const uint8_t*>(b_scales);
-  a.y = y;
-  a.y_ld = y_ld;
-  a.M = M;
-  a.N = N;
-  a.K = K;
-  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(K), 64));
-  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(K), kFp4BlockK));
-  a.scale_tiles = static_cast<int>(fp4_scale_tiles(K, format));
-  a.alpha = alpha;
-  a.bf16 = dtype == ASHQK_BF16;
-  return encode_tensor_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(b_codes), fp4_padded_k(K) / 2, N, b_ld,
-                              128, kTileN, CU_TENSOR_MAP_SWIZZLE_128B);
+int encode_rows(CUtensorMap* map, const Fp4Matrix& m, int K, int box_rows) {
+  return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(m.codes), fp4_padded_k(K) / 2,
+                              m.rows, m.ld, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int rows_args(RowsArgs& a, RowsMaps& maps, const Fp4Product& p) {
+  a.ws = p.b.scales;
+  a.y = p.y;
+  a.y_ld = p.y_ld;
+  a.M = p.a.rows;
+  a.N = p.b.rows;
+  a.K = p.K;
+  a.k_steps = static_cast<int>(ceil_div64(fp4_padded_k(p.K), 64));
+  a.num_kb = static_cast<int>(ceil_div64(fp4_padded_k(p.K), kFp4BlockK));
+  a.scale_tiles = static_cast<int>(fp4_scale_tiles(p.K, p.format));
+  a.alpha = p.alpha;
+  a.bf16 = p.dtype == ASHQK_BF16;
+  return encode_rows(&maps.w, p.b, p.K, kTileN);
 }
 
 }  // namespace
 
-int fp4_matmul_rows(const void* a_codes, int64_t a_ld, const void* a_scales, const void* b_codes, int64_t b_ld,
-                    const void* b_scales, void* y, int64_t y_ld, int dtype, int M, int N, int K, int format, float alpha,
-                    cudaStream_t stream) {
+int fp4_matmul_rows(const Fp4Product& p, cudaStream_t stream) {
   int nt = 8;
-  while (nt < M && nt < 128) nt *= 2;
+  while (nt < p.a.rows && nt < 128) nt *= 2;
   RowsMaps maps;
   RowsArgs a = {};
-  int rc = rows_args(a, maps, b_codes, b_ld, b_scales, y, y_ld, dtype, M, N, K, format, alpha);
-  if (!rc)
-    rc = encode_tensor_map_2d(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<void*>(a_codes), fp4_padded_k(K) / 2, M, a_ld,
-                              128, nt, CU_TENSOR_MAP_SWIZZLE_128B);
+  int rc = rows_args(a, maps, p);
+  if (!rc) rc = encode_rows(&maps.x, p.a, p.K, nt);
   if (rc) return rc;
-  a.xs = static_cast<const uint8_t*>(a_scales);
-  return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, false, stream)
-                               : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, false, stream);
+  a.xs = p.a.scales;
+  return p.format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, false, stream)
+                                 : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, false, stream);
 }
 
 // Whether w4a4_linear quantises x inside the product: up to 32 rows, of a length whose slice fits beside the ring (an
@@ -587,29 +596,28 @@ bool fp4_fused_ok(int M, int N, int K) {
   return M <= 16 ? K <= 32768 && work <= (1 << 24) : M <= 32 && K <= 16384 && work <= (6 << 20);
 }
 
-int fp4_linear_rows(const void* x, int64_t x_ld, int dtype, bool gated, float x_gs, const void* w_codes, int64_t w_ld,
-                    const void* w_scales, void* y, int64_t y_ld, int M, int N, int K, int format, float alpha,
-                    cudaStream_t stream) {
+int fp4_linear_rows(const Fp4Source& x, const Fp4Product& p, cudaStream_t stream) {
   RowsMaps maps;
   RowsArgs a = {};
-  const int rc = rows_args(a, maps, w_codes, w_ld, w_scales, y, y_ld, dtype, M, N, K, format, alpha);
-  if (rc) return rc;
+  if (const int rc = rows_args(a, maps, p)) return rc;
   maps.x = maps.w;  // not used
-  a.x = x;
-  a.x_ld = x_ld;
-  a.xq = fp4_quant_params(x_gs);
-  a.gated = gated;
-  a.align = std::min(chunk_align(x, x_ld, 2), gated ? chunk_align(nullptr, K, 2) : 32);
+  a.x = x.x;
+  a.x_ld = x.ld;
+  a.xq = fp4_quant_params(x.gs);
+  a.gated = x.gated;
+  a.align = std::min(chunk_align(x.x, x.ld, 2), x.gated ? chunk_align(nullptr, p.K, 2) : 32);
+  const int M = p.a.rows;
   const int nt = M <= 8 ? 8 : M <= 16 ? 16 : 32;
-  return format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, true, stream)
-                               : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, true, stream);
+  return p.format == ASHQK_MXFP4 ? launch_rows_fmt<ASHQK_MXFP4>(maps, a, nt, true, stream)
+                                 : launch_rows_fmt<ASHQK_NVFP4>(maps, a, nt, true, stream);
 }
 
 }  // namespace ashqk
 
 extern "C" int ashqk_fp4_set_tuning(int cluster, int ring, int split) {
   if (split < 0 || split > 2) return ASHQK_ERR_INVALID_ARGUMENT;
-  if (cluster < 0 || cluster > ashqk::kMaxCluster || ring < 0 || ring == 1 || ring > ashqk::kMaxRing) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (cluster < 0 || cluster > ashqk::kMaxCluster || ring < 0 || ring == 1 || ring > ashqk::kMaxRing)
+    return ASHQK_ERR_INVALID_ARGUMENT;
   ashqk::g_cluster.store(cluster, std::memory_order_relaxed);
   ashqk::g_ring.store(ring, std::memory_order_relaxed);
   ashqk::fp4_set_pair_split(split);

@@ -37,8 +37,8 @@ constexpr int kChunk = 32;  // columns per thread
 template <int FMT, typename T, bool GATED, bool WHOLE>
 __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : GATED ? 3 : 4)
     quantize_fp4_kernel(const T* x, int64_t x_ld, uint8_t* __restrict__ codes, uint32_t codes_ld,
-                        uint8_t* __restrict__ scales, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks, Fp4Quant q,
-                        int align, int early) {
+                        uint8_t* __restrict__ scales, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks,
+                        Fp4Quant q, int align, int early) {
   constexpr int kHalves = kChunk / 16;
   constexpr int kBlocks = kChunk / fp4_block(FMT);  // of a chunk
   pdl_wait();
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : GATED ? 3 
   }
   if (i >= total) return;
   *reinterpret_cast<uint4*>(codes + row * codes_ld + chunk * (kChunk / 2)) = make_uint4(c[0].x, c[0].y, c[1].x, c[1].y);
-  uint8_t* s = scales + ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+  uint8_t* s = scales + fp4_scale_offset(row, block, tiles);
   if (WHOLE) {
     if ((block & 3) == 0) *reinterpret_cast<uint32_t*>(s) = bytes;
   } else {
@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : GATED ? 3 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_rows_kernel(const uint8_t* codes, uint32_t codes_ld, const uint8_t* scales, T* __restrict__ out,
-                           int64_t out_ld, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks, float gs, bool wide) {
+                           int64_t out_ld, uint32_t tiles, uint32_t total, int K, FastDiv by_chunks, float gs,
+                           bool wide) {
   constexpr int kBlocks = kChunk / fp4_block(FMT);
   pdl_wait();
   const uint32_t i = blockIdx.x * kQuantThreads + threadIdx.x;
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(kQuantThreads)
   const uint32_t chunk = i - row * by_chunks.d;
   const uint32_t block = chunk * kBlocks;
   const uint4 c4 = ld_once_v4(codes + row * codes_ld + chunk * (kChunk / 2));
-  const uint8_t* s = scales + ((row >> 7) * tiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+  const uint8_t* s = scales + fp4_scale_offset(row, block, tiles);
   const uint32_t bytes = kBlocks == 1 ? *s : *reinterpret_cast<const uint16_t*>(s);
   const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
   T* y = out + row * out_ld + chunk * kChunk;
@@ -154,14 +155,16 @@ __global__ void __launch_bounds__(kQuantThreads)
 #pragma unroll
       for (int j = 0; j < static_cast<int>(4 * sizeof(T)); j += 8)
         asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(reinterpret_cast<uint32_t*>(o) + j),
-                     "r"(w[j]), "r"(w[j + 1]), "r"(w[j + 2]), "r"(w[j + 3]), "r"(w[j + 4]), "r"(w[j + 5]), "r"(w[j + 6]), "r"(w[j + 7])
+                     "r"(w[j]), "r"(w[j + 1]), "r"(w[j + 2]), "r"(w[j + 3]), "r"(w[j + 4]), "r"(w[j + 5]), "r"(w[j + 6]),
+                     "r"(w[j + 7])
                      : "memory");
     } else {
       constexpr int kPer = 16 / sizeof(T);  // values in 16 bytes
 #pragma unroll
       for (int j = 0; j < 16; j += kPer) {
+        const uint32_t* q = w + 4 * (j / kPer);
         if (n >= j + kPer)
-          *reinterpret_cast<uint4*>(o + j) = make_uint4(w[4 * (j / kPer)], w[4 * (j / kPer) + 1], w[4 * (j / kPer) + 2], w[4 * (j / kPer) + 3]);
+          *reinterpret_cast<uint4*>(o + j) = make_uint4(q[0], q[1], q[2], q[3]);
         else
 #pragma unroll
           for (int k = 0; k < kPer; ++k)
@@ -171,8 +174,9 @@ __global__ void __launch_bounds__(kQuantThreads)
   }
 }
 
-// Rows of any alignment. One thread writes eight columns from a 16-byte boundary of the output on: where rows start `mis` values behind one, those are the
-// last `mis` of code word c - 1 and the first of word c (eight codes, all of one block, each).
+// Rows of any alignment. One thread writes eight columns from a 16-byte boundary of the output on: where rows start
+// `mis` values behind one, those are the last `mis` of code word c - 1 and the first of word c (eight codes, all of
+// one block, each).
 template <int FMT, typename T, int BATCH>
 __global__ void __launch_bounds__(kQuantThreads)
     dequantize_fp4_kernel(const uint8_t* codes, int64_t codes_ld, const uint8_t* scales, T* __restrict__ out,
@@ -198,11 +202,11 @@ __global__ void __launch_bounds__(kQuantThreads)
       const uint32_t* w = reinterpret_cast<const uint32_t*>(codes + row * codes_ld);
       if (c < words) {
         c1[b] = w[c];
-        s1[b] = scales[fp4_scale_offset(row, c * 8 / fp4_block(FMT), tiles)];
+        s1[b] = scales[fp4_scale_offset(row, static_cast<uint32_t>(c) * 8 / fp4_block(FMT), tiles)];
       }
       if (mis[b] && c > 0) {
         c0[b] = w[c - 1];
-        s0[b] = scales[fp4_scale_offset(row, (c - 1) * 8 / fp4_block(FMT), tiles)];
+        s0[b] = scales[fp4_scale_offset(row, static_cast<uint32_t>(c - 1) * 8 / fp4_block(FMT), tiles)];
       }
     }
   }
@@ -258,34 +262,42 @@ int for_slabs(int64_t rows, int64_t most, F launch) {
   return ASHQK_OK;
 }
 
+// Where a quantiser's result goes.
+struct Fp4Target {
+  uint8_t* codes;
+  int64_t ld;
+  uint8_t* scales;
+  int M, K;
+  bool early;
+  cudaStream_t stream;
+};
+
 template <int FMT, typename T, bool GATED, bool WHOLE>
-int quantize_launch(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
-                    bool early, cudaStream_t stream) {
-  int align = chunk_align(x, x_ld, sizeof(T));
-  if (GATED) align = std::min(align, chunk_align(nullptr, K, sizeof(T)));
-  const int64_t chunks = fp4_padded_k(K) / kChunk;
-  const int64_t tiles = fp4_scale_tiles(K, FMT);
-  return for_slabs(M, ((1ll << 31) - 1) / codes_ld, [&](int64_t row0, int64_t rows) {
-    return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, WHOLE>, ceil_div64(rows * chunks, kQuantThreads), kQuantThreads,
-                      stream, static_cast<const T*>(x) + row0 * x_ld, x_ld, codes + row0 * codes_ld, codes_ld,
-                      scales + row0 / kFp4TileRows * tiles * kFp4TileBytes, tiles, rows * chunks, K,
-                      fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(gs), align, early);
+int quantize_launch(const Fp4Source& x, const Fp4Target& t) {
+  int align = chunk_align(x.x, x.ld, sizeof(T));
+  if (GATED) align = std::min(align, chunk_align(nullptr, t.K, sizeof(T)));
+  const int64_t chunks = fp4_padded_k(t.K) / kChunk;
+  const int64_t tiles = fp4_scale_tiles(t.K, FMT);
+  return for_slabs(t.M, ((1ll << 31) - 1) / t.ld, [&](int64_t row0, int64_t rows) {
+    return launch_pdl(quantize_fp4_kernel<FMT, T, GATED, WHOLE>, ceil_div64(rows * chunks, kQuantThreads),
+                      kQuantThreads, t.stream, static_cast<const T*>(x.x) + row0 * x.ld, x.ld, t.codes + row0 * t.ld,
+                      t.ld, t.scales + row0 / kFp4TileRows * tiles * kFp4TileBytes, tiles, rows * chunks, t.K,
+                      fast_div(static_cast<uint32_t>(chunks)), fp4_quant_params(x.gs), align, t.early);
   });
 }
 
-template <int FMT, typename T, bool GATED>
-int quantize_shaped(const void* x, int64_t x_ld, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, float gs,
-                    bool early, cudaStream_t stream) {
-  const bool whole = fp4_padded_k(K) % (4 * fp4_block(FMT)) == 0;
-  return (whole ? quantize_launch<FMT, T, GATED, true> : quantize_launch<FMT, T, GATED, false>)(
-      x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
+template <int FMT, typename T>
+int quantize_typed(const Fp4Source& x, const Fp4Target& t) {
+  const bool whole = fp4_padded_k(t.K) % (4 * fp4_block(FMT)) == 0;
+  if (x.gated) return whole ? quantize_launch<FMT, T, true, true>(x, t) : quantize_launch<FMT, T, true, false>(x, t);
+  return whole ? quantize_launch<FMT, T, false, true>(x, t) : quantize_launch<FMT, T, false, false>(x, t);
 }
 
-template <int FMT, typename T>
-int quantize_typed(const void* x, int64_t x_ld, bool gated, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M,
-                   int K, float gs, bool early, cudaStream_t stream) {
-  return gated ? quantize_shaped<FMT, T, true>(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream)
-               : quantize_shaped<FMT, T, false>(x, x_ld, codes, codes_ld, scales, M, K, gs, early, stream);
+template <int FMT>
+int quantize_format(const Fp4Source& x, const Fp4Target& t) {
+  return x.dtype == ASHQK_F16    ? quantize_typed<FMT, __half>(x, t)
+         : x.dtype == ASHQK_BF16 ? quantize_typed<FMT, __nv_bfloat16>(x, t)
+                                 : quantize_typed<FMT, float>(x, t);
 }
 
 template <int FMT, typename T>
@@ -326,21 +338,10 @@ bool fp4_global_scale_ok(int format, float gs) {
   return format == ASHQK_MXFP4 ? gs == 1.0f : gs >= 1e-18f && gs <= 1e18f;
 }
 
-// `early`: let the next launch start while this one runs. Only for a consumer that reads the result
-// behind its own griddepcontrol.wait, which a product reading these codes as weights does not.
-int quantize_fp4(const void* x, int64_t x_ld, int dtype, bool gated, void* codes, int64_t codes_ld, void* scales, int M,
-                 int K, int format, float gs, bool early, cudaStream_t stream) {
-  uint8_t* c = static_cast<uint8_t*>(codes);
-  uint8_t* s = static_cast<uint8_t*>(scales);
-#define ASHQK_QUANT(FMT, T) quantize_typed<FMT, T>(x, x_ld, gated, c, codes_ld, s, M, K, gs, early, stream)
-  if (format == ASHQK_MXFP4)
-    return dtype == ASHQK_F16    ? ASHQK_QUANT(ASHQK_MXFP4, __half)
-           : dtype == ASHQK_BF16 ? ASHQK_QUANT(ASHQK_MXFP4, __nv_bfloat16)
-                                 : ASHQK_QUANT(ASHQK_MXFP4, float);
-  return dtype == ASHQK_F16    ? ASHQK_QUANT(ASHQK_NVFP4, __half)
-         : dtype == ASHQK_BF16 ? ASHQK_QUANT(ASHQK_NVFP4, __nv_bfloat16)
-                               : ASHQK_QUANT(ASHQK_NVFP4, float);
-#undef ASHQK_QUANT
+int quantize_fp4(const Fp4Source& x, uint8_t* codes, int64_t codes_ld, uint8_t* scales, int M, int K, int format, bool early,
+                 cudaStream_t stream) {
+  const Fp4Target t = {codes, codes_ld, scales, M, K, early, stream};
+  return format == ASHQK_MXFP4 ? quantize_format<ASHQK_MXFP4>(x, t) : quantize_format<ASHQK_NVFP4>(x, t);
 }
 
 }  // namespace ashqk
@@ -348,7 +349,8 @@ int quantize_fp4(const void* x, int64_t x_ld, int dtype, bool gated, void* codes
 using namespace ashqk;
 
 extern "C" int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int64_t* scales_bytes) {
-  if (M < 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format) || !codes_ld || !scales_bytes) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (M < 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format) || !codes_ld || !scales_bytes)
+    return ASHQK_ERR_INVALID_ARGUMENT;
   *codes_ld = fp4_padded_k(K) / 2;
   *scales_bytes = ceil_div64(M, kFp4TileRows) * fp4_scale_tiles(K, format) * kFp4TileBytes;
   return ASHQK_OK;
@@ -357,20 +359,21 @@ extern "C" int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int6
 extern "C" int ashqk_quantize_fp4(const void* x, int64_t x_ld, int dtype, int gated, void* codes, int64_t codes_ld,
                                   void* scales, int M, int K, int format, float global_scale, void* stream) {
   const int size = dtype_size(dtype);
-  if (!x || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(x, size) || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
+  if (!x || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(x, size) || !fp4_format_ok(format))
+    return ASHQK_ERR_INVALID_ARGUMENT;
   if (x_ld < static_cast<int64_t>(K) * (gated ? 2 : 1) || !fp4_global_scale_ok(format, global_scale))
     return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(codes, codes_ld, scales, K)) return rc;
-  return quantize_fp4(x, x_ld, dtype, gated != 0, codes, codes_ld, scales, M, K, format, global_scale, false,
-                      static_cast<cudaStream_t>(stream));
+  return quantize_fp4({x, x_ld, dtype, gated != 0, global_scale}, static_cast<uint8_t*>(codes), codes_ld,
+                      static_cast<uint8_t*>(scales), M, K, format, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ashqk_dequantize_fp4(const void* codes, int64_t codes_ld, const void* scales, void* out, int64_t out_ld,
                                     int dtype, int M, int K, int format, float global_scale, void* stream) {
   const int size = dtype_size(dtype);
-  if (!out || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(out, size) || !fp4_format_ok(format) || out_ld < K ||
-      !fp4_global_scale_ok(format, global_scale))
+  if (!out || M <= 0 || K <= 0 || K > kFp4MaxK || !size || !aligned(out, size) || !fp4_format_ok(format))
     return ASHQK_ERR_INVALID_ARGUMENT;
+  if (out_ld < K || !fp4_global_scale_ok(format, global_scale)) return ASHQK_ERR_INVALID_ARGUMENT;
   if (const int rc = check_fp4_operand(codes, codes_ld, scales, K)) return rc;
   const uint8_t* c = static_cast<const uint8_t*>(codes);
   const uint8_t* s = static_cast<const uint8_t*>(scales);
