@@ -76,7 +76,7 @@ int quantize_fp4(const Fp4Source& x, uint8_t* codes, int64_t codes_ld, uint8_t* 
                  cudaStream_t stream);
 int fp4_matmul_rows(const Fp4Product& p, cudaStream_t stream);
 int fp4_matmul_pair(const Fp4Product& p, cudaStream_t stream);
-bool fp4_fused_ok(int M, int N, int K);
+bool fp4_fused_ok(int M, int N, int K, bool gated);
 // p.a is not used but for its rows.
 int fp4_linear_rows(const Fp4Source& x, const Fp4Product& p, cudaStream_t stream);
 void fp4_set_pair_split(int split);

@@ -590,9 +590,10 @@ int fp4_matmul_rows(const Fp4Product& p, cudaStream_t stream) {
 // Measured (us, fused against two launches, in a graph): up to 16 rows, at M K tiles = 6.3 million 12.8 / 15.9
 // (8 rows 4096->24576) and 11.2 / 11.7 (16 rows 12288->4096), at 12.6 million 15.3 / 16.1 (16 rows 4096->24576;
 // NVFP4 17.2 / 17.2); with the wider instruction of 32 rows 8.4 / 9.3 at 4.2 million (4096->4096), 9.8 / 9.9 at 6.3
-// million (4096->6144), 13.2 / 12.7 at 9.4 million (24 rows 12288->4096).
-bool fp4_fused_ok(int M, int N, int K) {
-  const int64_t work = static_cast<int64_t>(M) * K * ceil_div(N, kTileN);
+// million (4096->6144), 13.2 / 12.7 at 9.4 million (24 rows 12288->4096). A gated value costs two loads, an
+// exponential and a quotient more and counts three times (12288->4096: 8 rows 11.2 fused, 16 rows 16.8 against 12.5).
+bool fp4_fused_ok(int M, int N, int K, bool gated) {
+  const int64_t work = static_cast<int64_t>(M) * K * ceil_div(N, kTileN) * (gated ? 3 : 1);
   return M <= 16 ? K <= 32768 && work <= (1 << 24) : M <= 32 && K <= 16384 && work <= (6 << 20);
 }
 

@@ -57,11 +57,11 @@ extern "C" int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a
   return fp4_matmul({a, b, K, format, alpha, y, y_ld, dtype}, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes) {
+extern "C" int ashqk_w4a4_workspace_size(int M, int N, int K, int format, int gated, size_t* bytes) {
   if (!bytes || M <= 0 || N <= 0 || K <= 0 || K > kFp4MaxK || !fp4_format_ok(format)) return ASHQK_ERR_INVALID_ARGUMENT;
   size_t offset;
   *bytes = 0;
-  if (!fp4_fused_ok(M, N, K)) workspace_layout(M, K, format, &offset, bytes);
+  if (!fp4_fused_ok(M, N, K, gated != 0)) workspace_layout(M, K, format, &offset, bytes);
   return ASHQK_OK;
 }
 
@@ -76,7 +76,7 @@ extern "C" int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gat
   const Fp4Source src = {x, x_ld, dtype, gated != 0, x_scale};
   const Fp4Matrix w = {static_cast<const uint8_t*>(w_codes), w_ld, static_cast<const uint8_t*>(w_scales), N};
   Fp4Product p = {{nullptr, 0, nullptr, M}, w, K, format, x_scale * w_scale, y, y_ld, dtype};
-  if (fp4_fused_ok(M, N, K)) return fp4_linear_rows(src, p, st);
+  if (fp4_fused_ok(M, N, K, src.gated)) return fp4_linear_rows(src, p, st);
   size_t offset, bytes;
   workspace_layout(M, K, format, &offset, &bytes);
   if (!workspace || workspace_bytes < bytes || !aligned(workspace, 16)) return ASHQK_ERR_WORKSPACE;

@@ -302,7 +302,7 @@ at::Tensor w4a4_linear(const at::Tensor& x, const at::Tensor& codes, const at::T
   at::Tensor y = new_cuda({r.rows, N}, x.scalar_type(), x.device());
   if (r.rows > 0 && N > 0) {
     size_t bytes = 0;
-    check_rc(ashqk_w4a4_workspace_size(static_cast<int>(r.rows), static_cast<int>(N), static_cast<int>(K), static_cast<int>(format), &bytes), "w4a4_linear");
+    check_rc(ashqk_w4a4_workspace_size(static_cast<int>(r.rows), static_cast<int>(N), static_cast<int>(K), static_cast<int>(format), gated, &bytes), "w4a4_linear");
     // Holds x quantised between two launches; from PyTorch's allocator, so streams and graphs each have their own.
     at::Tensor ws;
     if (bytes) ws = new_cuda({static_cast<int64_t>(bytes)}, at::kByte, x.device());

@@ -367,7 +367,7 @@ ASHQK_API int ashqk_fp4_matmul(const void* a_codes, int64_t a_ld, const void* a_
  * one launch; for more, the workspace of ashqk_w4a4_workspace_size bytes (16-byte aligned, contents
  * irrelevant, written) holds Q(x) between two launches.
  */
-ASHQK_API int ashqk_w4a4_workspace_size(int M, int N, int K, int format, size_t* bytes);
+ASHQK_API int ashqk_w4a4_workspace_size(int M, int N, int K, int format, int gated, size_t* bytes);
 ASHQK_API int ashqk_w4a4_linear(const void* x, int64_t x_ld, int dtype, int gated, float x_scale, const void* w_codes,
                                 int64_t w_ld, const void* w_scales, float w_scale, void* y, int64_t y_ld, int M, int N,
                                 int K, int format, void* workspace, size_t workspace_bytes, void* stream);

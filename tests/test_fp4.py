@@ -139,7 +139,7 @@ def _lib():
     lib.ashqk_dequantize_fp4.argtypes = [VP, I64, VP, VP, I64, CI, CI, CI, CI, CF, VP]
     lib.ashqk_fp4_matmul.argtypes = [VP, I64, VP, VP, I64, VP, VP, I64, CI, CI, CI, CI, CI, CF, VP]
     lib.ashqk_w4a4_linear.argtypes = [VP, I64, CI, CI, CF, VP, I64, VP, CF, VP, I64, CI, CI, CI, CI, VP, ctypes.c_size_t, VP]
-    lib.ashqk_w4a4_workspace_size.argtypes = [CI, CI, CI, CI, ctypes.POINTER(ctypes.c_size_t)]
+    lib.ashqk_w4a4_workspace_size.argtypes = [CI, CI, CI, CI, CI, ctypes.POINTER(ctypes.c_size_t)]
     return lib
 
 
@@ -154,7 +154,7 @@ def test_c_abi_sizes():
         assert lib.ashqk_fp4_sizes(m, k, fmt, ctypes.byref(ld), ctypes.byref(n)) == 1
     size = ctypes.c_size_t()
     for m, n_, k, fmt in ((0, 8, 32, 0), (1, 0, 32, 0), (1, 8, 0, 0), (1, 8, 32, 7)):
-        assert lib.ashqk_w4a4_workspace_size(m, n_, k, fmt, ctypes.byref(size)) == 1
+        assert lib.ashqk_w4a4_workspace_size(m, n_, k, fmt, 0, ctypes.byref(size)) == 1
 
 
 def test_c_abi_switches():
