@@ -16,6 +16,10 @@
 //               -> the shared memory of the CTA that adds these rows of A, counted in bytes on its barrier
 //               (st.async, or with 32 columns and more through own shared memory and bulk copies)
 //
+// Measured on a B200, launches back to back in a graph, x in fp16, MXFP4: one token 4096->6144 4.9 us, 4096->4096 4.7,
+// 4096->24576 11.7 (4.6 TB/s of weights), 12288->4096 7.6; sixteen 6.3, 5.7, 15.2, 10.9. A launch is latency from end
+// to end: 0.75 us until x is quantised, 0.2-0.3 per stage, 1 for the exchange, 0.85 to the next launch's start.
+//
 // The scales have two to eight buffers in TMEM: the copies of stage i wait for the MMAs of stage i - buffers. With
 // two, that wait and not the tensor core set the pace of narrow tiles. All waits are bounded.
 #include <algorithm>
