@@ -429,8 +429,17 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         __syncwarp();
       }
     }
-    cluster_arrive();
-    if (epilogue && my_groups > 0 && mbar_wait_cluster(received, 0, abort)) {
+    // The last barrier: no CTA leaves while another may still store into it, nor while a copy still reads what it sent.
+    // st.async takes its values from registers: issued, then arrived. A bulk copy reads the sender's shared memory until
+    // its bytes are counted, and only the receiver sees that: there every CTA arrives behind its own receipt, so that
+    // the barrier stands for all receipts and with them for every copy of every sender.
+    if (!L::kStaged) cluster_arrive();
+    const bool received_all = epilogue && my_groups > 0 && mbar_wait_cluster(received, 0, abort);
+    if (L::kStaged) {
+      __syncwarp();
+      cluster_arrive();
+    }
+    if (received_all) {
 #pragma unroll 2
       for (int l = turn; l < my_groups; l += 2) {
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -446,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
       }
     }
     __syncwarp();
-    cluster_wait();  // no CTA leaves while another may still store into it
+    cluster_wait();
   }
 }
 
