@@ -219,11 +219,12 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  // After the allocation: a CTA of the next launch that holds TMEM on this SM waits for this grid, which must
-  // not still be waiting for TMEM.
-  pdl_launch_dependents();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   pdl_wait();
+  // Behind the wait: what ran before this grid has then ended, also for a next launch that reads ahead of its own wait
+  // (the decode GEMV loads its weights there). And behind the allocation: a CTA of the next launch that holds TMEM on
+  // this SM waits for this grid, which must not still be waiting for TMEM.
+  pdl_launch_dependents();
 
   const uint32_t x_codes = sbase + a.off_x;
   const uint32_t x_scales = x_codes + static_cast<uint32_t>(kb1 - kb0) * L::kX;

@@ -46,3 +46,33 @@ def test_products_between_decode_calls(fmt, m, n):
     torch.cuda.synchronize()
     for i, y in got:
         assert torch.equal(y, want[i]), i
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("m", [1, 16, 32, 100, 300])
+@pytest.mark.parametrize("call", ["linear", "matmul", "gated", "quantize", "dequantize"])
+def test_awq_weights_written_before_a_call(fmt, m, call):
+    """AWQ weights written, a 4-bit floating-point call, a decode GEMV on those weights: no wait in between, and the GEMV
+    multiplies what was written."""
+    x, w = operands(m, 512, 1024, fmt, m)
+    q = ashqk.quantize_fp4(x, fmt)
+    x2 = x.repeat(1, 2)
+    between = {"linear": lambda: ashqk.w4a4_linear(x, w), "matmul": lambda: ashqk.fp4_matmul(q, w), "gated": lambda: ashqk.w4a4_linear(x2, w, gated=True),
+               "quantize": lambda: ashqk.quantize_fp4(x, fmt), "dequantize": lambda: ashqk.dequantize_fp4(q)}[call]
+    problems = [[torch.from_numpy(t).cuda() for t in O.make_problem(1, 16384, 4096, 128, seed=s)] for s in range(2)]
+    xa = problems[0][0]
+    want = [ashqk.w4a16_linear(xa, *p[1:]) for p in problems]
+    between()
+    qw, qz, s = (torch.empty_like(t) for t in problems[0][1:])
+    torch.cuda.synchronize()
+    got = []
+    for i in range(8):
+        _, nqw, nqz, ns = problems[i % 2]
+        qz.copy_(nqz)
+        s.copy_(ns)
+        qw.copy_(nqw)
+        between()
+        got.append(ashqk.w4a16_linear(xa, qw, qz, s))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % 2]), i
