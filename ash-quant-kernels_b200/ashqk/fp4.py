@@ -125,7 +125,8 @@ def quantize_fp4(x: torch.Tensor, format: str = "mxfp4", *, global_scale: float 
 def silu_mul_quantize_fp4(gate_up: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
     """gate_up [..., 2 K] -> FP4Tensor of silu(gate) * up, gate and up the two halves of the last dimension.
 
-    The activation is computed in fp32 and rounded once, to the format: one pass over gate_up.
+    The activation is computed in fp32, off by at most 2^-20 + 2^-23 |gate| of itself, and then rounded to the format: one
+    pass over gate_up.
     """
     k = gate_up.shape[-1]
     assert k % 2 == 0, "gate and up are the two halves of the last dimension"

@@ -383,9 +383,30 @@ __device__ __forceinline__ uint32_t abs_max16(const Raw16<T>& r) {
   }
 }
 
-// silu(gate) * up in fp32. exp overflows to infinity for gates below -88 and the quotient is then 0.
-__device__ __forceinline__ float silu_mul(float gate, float up) {
-  return __fdividef(gate, 1.0f + __expf(-gate)) * up;
+// silu(gate) * up in fp32: with h = exp(-|gate| / 2), gate up / (1 + h^2) for gates from 0 on, (gate h) (up h) / (1 + h^2)
+// below. The denominator is in [1, 2] and each factor h meets an operand first, so nothing overflows or vanishes on the
+// way while the result is a normal number: exp(-gate) itself is infinite from a gate of -88.7 on, where a large `up`
+// still gives one. Relative error at most 2^-20 + 2^-23 |gate|: h twice (the exponent's rounding and its constant's, 0.8
+// |gate| 2^-24 each time, and two units of ex2.approx), the reciprocal, five roundings. Gates below -174 give 0 (less than
+// 2^-116 in truth).
+//
+// Sixteen values, v[i] = silu(v[i]) * up[i], the products in pairs: 8192 x 12288 to MXFP4 72 us, one by one 75.
+__device__ __forceinline__ void silu_mul16(float* v, const float* up) {
+  constexpr float kHalfLog2E = 0.72134752044448170f;
+#pragma unroll
+  for (int i = 0; i < 16; i += 2) {
+    float h[2], a[2], den[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h[j]) : "f"(fabsf(v[i + j]) * -kHalfLog2E));
+      a[j] = v[i + j] < 0.0f ? h[j] : 1.0f;
+    }
+    const uint64_t h2 = f32x2(h[0], h[1]), a2 = f32x2(a[0], a[1]);
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(den[0]), "=f"(den[1]) : "l"(fma2(h2, h2, f32x2(1.0f, 1.0f))));
+    const uint64_t r2 = f32x2(reciprocal_approx(den[0]), reciprocal_approx(den[1]));
+    const uint64_t y = mul2(mul2(mul2(f32x2(v[i], v[i + 1]), a2), r2), mul2(f32x2(up[i], up[i + 1]), a2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(y));
+  }
 }
 
 }  // namespace ashqk

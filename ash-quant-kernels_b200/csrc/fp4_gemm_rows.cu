@@ -136,8 +136,7 @@ __device__ __forceinline__ void quantize_slice(const RowsArgs& a, int kb0, int k
       if constexpr (GATED) {
         float w[16];
         unpack16<T>(u[b], w);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = silu_mul(v[j], w[j]);
+        silu_mul16(v, w);
         amax = abs_max16(v);
       } else {
         amax = abs_max16(g[b]);

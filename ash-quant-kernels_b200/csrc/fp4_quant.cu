@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(kQuantThreads, sizeof(T) == 4 ? 2 : GATED ? 3 
     if constexpr (GATED) {
       float w[16];
       unpack16<T>(u[h], w);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[16 * h + j] = silu_mul(v[16 * h + j], w[j]);
+      silu_mul16(v + 16 * h, w);
       amax[h] = abs_max16(v + 16 * h);
     } else {
       amax[h] = abs_max16(g[h]);

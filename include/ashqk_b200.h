@@ -342,7 +342,8 @@ ASHQK_API int ashqk_fp4_sizes(int M, int K, int format, int64_t* codes_ld, int64
 
 /*
  * x [M, K] (ashqk_dtype, row stride x_ld elements) -> codes, scales. With gated != 0, x is [M, 2 K] and
- * what is quantised is silu(x[:, :K]) * x[:, K:], computed in fp32 and rounded once, to the format.
+ * what is quantised is silu(x[:, :K]) * x[:, K:], computed in fp32 (off by at most 2^-20 + 2^-23 |gate| of itself before
+ * it is rounded to the format; values below 2^-116 may become 0).
  */
 ASHQK_API int ashqk_quantize_fp4(const void* x, int64_t x_ld, int dtype, int gated, void* codes, int64_t codes_ld,
                                  void* scales, int M, int K, int format, float global_scale, void* stream);
