@@ -105,11 +105,18 @@ class FP4Tensor:
 
 def fp4_global_scale(x: torch.Tensor) -> float:
     """The NVFP4 global scale that maps the largest magnitude of x onto the largest value of the format
-    (amax / (448 * 6)); 1 for a tensor of zeros. Copies one number to the host."""
+    (amax / (448 * 6)); 1 for a tensor of zeros. Copies one number to the host.
+
+    A global scale is at least 1e-18, which tensors with an amax below 2.7e-15 get (blocks under 6e-21 become 0 with it),
+    and at most 1e18: a larger amax than 2.7e21 is an error.
+    """
     amax = float(x.detach().abs().amax()) if x.numel() else 0.0
     assert math.isfinite(amax), "x holds an infinity or a NaN"
+    if amax == 0.0:
+        return 1.0
     g = float(torch.tensor(amax / (_E4M3_MAX * _E2M1_MAX), dtype=torch.float32))
-    return g if g >= 1e-18 else 1.0
+    assert g <= 1e18, f"largest magnitude {amax} is beyond what NVFP4 with a global scale of 1e18 holds"
+    return max(g, 1e-18)
 
 
 def quantize_fp4(x: torch.Tensor, format: str = "mxfp4", *, global_scale: float = 1.0) -> FP4Tensor:
