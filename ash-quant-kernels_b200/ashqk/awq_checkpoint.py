@@ -14,7 +14,7 @@ from __future__ import annotations
 import json
 import os
 from dataclasses import dataclass
-from typing import Dict, Iterable, Optional
+from typing import Dict, Iterable, Mapping, Optional
 
 import torch
 
@@ -176,11 +176,14 @@ class AWQLinear(torch.nn.Module):
                 f"group_size={self.in_features // self.scales.shape[0]}, bias={self.bias is not None}")
 
 
-def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer], fp4_format: Optional[str] = None) -> list[str]:
+def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer], fp4_format: Optional[str] = None,
+                          input_global_scales: Optional[Mapping[str, float]] = None) -> list[str]:
     """Swap each ``nn.Linear`` of ``model`` named in ``layers`` for an ``AWQLinear``.
 
     With ``fp4_format`` ("mxfp4" or "nvfp4") for an ``FP4Linear`` instead: the checkpoint's weights, quantised again
-    to 4-bit floating point, times activations quantised as they come (layers on the GPU).
+    to 4-bit floating point, times activations quantised as they come (layers on the GPU). "nvfp4" wants the global
+    scale of each layer's input, by the layer's name: ``fp4_global_scale`` of inputs that the layer has seen. Without
+    them it is 1, which small activations do not survive, and there is a warning.
 
     Names follow ``model.named_modules()``. The quantised layer must have the Linear's in/out
     features. Returns the replaced names; layers of the checkpoint that match no module are an error.
@@ -189,6 +192,22 @@ def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer], f
     missing = [n for n in layers if n not in modules]
     if missing:
         raise KeyError(f"checkpoint layers with no module in the model: {missing[:5]}")
+    if input_global_scales is not None:
+        if fp4_format != "nvfp4":
+            raise ValueError(f"input_global_scales belong to 'nvfp4', not to {fp4_format!r}")
+        if set(input_global_scales) != set(layers):
+            raise KeyError(f"input_global_scales and layers differ in {sorted(set(input_global_scales) ^ set(layers))[:5]}")
+        bad = {n: g for n, g in input_global_scales.items() if not 1e-18 <= g <= 1e18}
+        if bad:
+            raise ValueError(f"input_global_scales outside 1e-18 .. 1e18: {bad}")
+
+    def convert(name: str, layer: AWQLayer) -> torch.nn.Module:
+        if not fp4_format:
+            return AWQLinear.from_layer(layer)
+        if input_global_scales is None:
+            return FP4Linear.from_awq(layer, fp4_format)
+        return FP4Linear.from_awq(layer, fp4_format, input_global_scale=input_global_scales[name])
+
     replaced = []
     for name, layer in layers.items():
         mod = modules[name]
@@ -199,6 +218,6 @@ def replace_linear_layers(model: torch.nn.Module, layers: Dict[str, AWQLayer], f
                              f"{mod.in_features}->{mod.out_features}")
         parent_name, _, child = name.rpartition(".")
         parent = modules[parent_name] if parent_name else model
-        setattr(parent, child, FP4Linear.from_awq(layer, fp4_format) if fp4_format else AWQLinear.from_layer(layer))
+        setattr(parent, child, convert(name, layer))
         replaced.append(name)
     return replaced

@@ -16,6 +16,7 @@ No reference counterpart: the reference multiplies 4-bit weights in 16 bits.
 from __future__ import annotations
 
 import math
+import warnings
 
 import torch
 
@@ -168,7 +169,9 @@ def w4a4_linear(x: torch.Tensor, weight: FP4Tensor, *, global_scale: float = 1.0
 class FP4Linear(torch.nn.Module):
     """A linear layer y = Q(x) @ W^T (+ bias) with W [out, in] held as an ``FP4Tensor``; CUDA only.
 
-    The W4A4 counterpart of ``AWQLinear``. ``input_global_scale`` is x's, for "nvfp4"; ``gated`` as in ``w4a4_linear``.
+    The W4A4 counterpart of ``AWQLinear``; ``gated`` as in ``w4a4_linear``. ``input_global_scale`` is x's, for "nvfp4": take
+    ``fp4_global_scale`` of inputs that the layer has seen. With 1 a block of x whose largest magnitude is below 6 * 2^-10
+    (0.006) becomes zeros, one below 6 * 2^-6 (0.09) has a scale of less than four bits and one above 2688 is cut off.
     """
 
     def __init__(self, weight: FP4Tensor, bias: torch.Tensor | None = None, *, input_global_scale: float = 1.0, gated: bool = False):
@@ -184,8 +187,12 @@ class FP4Linear(torch.nn.Module):
 
     @staticmethod
     def from_float(weight: torch.Tensor, bias: torch.Tensor | None = None, format: str = "nvfp4", **kwargs) -> "FP4Linear":
-        """From a dense weight [out, in] on the GPU; for "nvfp4" the global scale is ``fp4_global_scale(weight)``."""
+        """From a dense weight [out, in] on the GPU; for "nvfp4" the global scale is ``fp4_global_scale(weight)``, and
+        without an ``input_global_scale`` for x there is a warning."""
         g = fp4_global_scale(weight) if format == "nvfp4" else 1.0
+        if format == "nvfp4" and "input_global_scale" not in kwargs:
+            warnings.warn("nvfp4 without input_global_scale: with 1, blocks of x below 0.006 become zeros and those above 2688 are "
+                          "cut off; pass fp4_global_scale of inputs that the layer has seen", stacklevel=2)
         return FP4Linear(quantize_fp4(weight.detach(), format, global_scale=g), bias, **kwargs)
 
     @staticmethod

@@ -27,3 +27,47 @@ def test_global_scale_refuses_what_no_scale_holds():
         with pytest.raises(AssertionError, match="beyond"):
             ashqk.fp4_global_scale(torch.tensor([0.0, -amax]))
     assert ashqk.fp4_global_scale(torch.zeros(3, dtype=torch.float16)) == 1.0
+
+
+def _two_layers():
+    from ashqk.awq_checkpoint import AWQLayer
+
+    layer = AWQLayer(torch.zeros(128, 4, dtype=torch.int32), torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, 32, dtype=torch.float16), None)
+    model = torch.nn.Sequential()
+    for name in ("a", "b"):
+        model.add_module(name, torch.nn.Linear(128, 32))
+    return model, {"a": layer, "b": layer}
+
+
+def test_input_scales_reach_the_layers(monkeypatch):
+    from ashqk.awq_checkpoint import replace_linear_layers
+
+    model, layers = _two_layers()
+    seen = []
+    monkeypatch.setattr(ashqk.FP4Linear, "from_awq", staticmethod(lambda layer, fmt, **kw: seen.append((fmt, kw)) or torch.nn.Identity()))
+    assert replace_linear_layers(model, layers, "nvfp4", {"a": 0.25, "b": 0.5}) == ["a", "b"]
+    assert seen == [("nvfp4", {"input_global_scale": 0.25}), ("nvfp4", {"input_global_scale": 0.5})]
+
+
+@pytest.mark.parametrize("fmt,scales,error", [("nvfp4", {"a": 0.25}, KeyError), ("nvfp4", {"a": 1.0, "b": 1.0, "c": 1.0}, KeyError),
+                                              ("nvfp4", {"a": 0.25, "b": 0.0}, ValueError), ("nvfp4", {"a": float("nan"), "b": 1.0}, ValueError),
+                                              ("mxfp4", {"a": 1.0, "b": 1.0}, ValueError), (None, {"a": 1.0, "b": 1.0}, ValueError)])
+def test_input_scales_that_do_not_fit_replace_nothing(fmt, scales, error):
+    from ashqk.awq_checkpoint import replace_linear_layers
+
+    model, layers = _two_layers()
+    with pytest.raises(error):
+        replace_linear_layers(model, layers, fmt, scales)
+    assert all(type(m) is torch.nn.Linear for m in model)
+
+
+def test_conversion_without_an_input_scale_warns(monkeypatch):
+    w = ashqk.FP4Tensor(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8), (8, 64), "nvfp4", 0.5)
+    monkeypatch.setattr(ashqk.fp4, "quantize_fp4", lambda *a, **kw: w)
+    with pytest.warns(UserWarning, match="input_global_scale"):
+        assert ashqk.FP4Linear.from_float(torch.ones(8, 64)).input_global_scale == 1.0
+    import warnings
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        assert ashqk.FP4Linear.from_float(torch.ones(8, 64), input_global_scale=0.25).input_global_scale == 0.25
