@@ -71,7 +71,7 @@ class FP4Tensor:
     @staticmethod
     def from_rowmajor(codes: torch.Tensor, scales: torch.Tensor, format: str = "mxfp4", global_scale: float = 1.0) -> "FP4Tensor":
         """From a checkpoint's plain layout: codes uint8 [rows, K / 2], scales [rows, K / block] (uint8, or float8
-        of the format's kind). K is a multiple of the block."""
+        of the format's kind; E4M3 scales without a sign). K is a multiple of the block."""
         _check(format, global_scale)
         block = _BLOCK[format]
         assert codes.dtype == torch.uint8 and codes.dim() == 2 and scales.dim() == 2
@@ -81,6 +81,8 @@ class FP4Tensor:
             scales = scales.view(torch.uint8)
         assert k % block == 0 and k > 0 and scales.shape == (rows, k // block), \
             f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not {format} of one matrix"
+        # The tensor core takes E4M3 scales as unsigned, so a sign would count in dequantize_fp4 alone.
+        assert format == "mxfp4" or not bool((scales > 127).any()), "nvfp4 scales must not be negative"
         kp = -(-k // 32) * 32
         blocks = kp // block
         codes = torch.nn.functional.pad(codes, (0, (kp - k) // 2)).contiguous()

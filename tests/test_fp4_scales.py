@@ -71,3 +71,16 @@ def test_conversion_without_an_input_scale_warns(monkeypatch):
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         assert ashqk.FP4Linear.from_float(torch.ones(8, 64), input_global_scale=0.25).input_global_scale == 0.25
+
+
+def test_negative_block_scales_are_refused():
+    codes = torch.zeros(3, 32, dtype=torch.uint8)
+    scales = torch.ones(3, 4)
+    scales[2, 1] = -0.5
+    for bad in (scales.to(torch.float8_e4m3fn), scales.to(torch.float8_e4m3fn).view(torch.uint8)):
+        with pytest.raises(AssertionError, match="negative"):
+            ashqk.FP4Tensor.from_rowmajor(codes, bad, "nvfp4")
+    ashqk.FP4Tensor.from_rowmajor(codes, torch.full((3, 2), 200, dtype=torch.uint8), "mxfp4")  # E8M0 has no sign
+    nan = torch.full((3, 4), 127, dtype=torch.uint8)
+    assert int(ashqk.FP4Tensor.from_rowmajor(codes, nan, "nvfp4").scales_rowmajor().min()) == 127
+    ashqk.FP4Tensor.from_rowmajor(codes[:0], nan[:0], "nvfp4")
