@@ -78,6 +78,7 @@ struct RowsShape {
   // the sums go there by way of the own ring.
   static constexpr bool kOwnSlots = NT <= 32;
   static constexpr bool kStaged = NT >= 32;
+  static_assert(kOwnSlots || kStaged, "this CTA's own sums need a place");
   static constexpr uint32_t kStaging = NT / 4 * kTileN * 16;
   static constexpr uint32_t slots(int cluster) {
     return static_cast<uint32_t>(((NT / 4 + cluster - 1) / cluster) * cluster) * kTileN * 16;
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp4_rows_kernel(const __grid_cons
         } else {
           const int l = g / C, owner = g - l * C;
           const uint4 v = make_uint4(r[4 * h], r[4 * h + 1], r[4 * h + 2], r[4 * h + 3]);
-          if (owner == rank && (L::kOwnSlots || !L::kStaged))
+          if (owner == rank && L::kOwnSlots)
             sts_v4(slot(l, rank), v);
           else if (L::kStaged)
             sts_v4(sbase + static_cast<uint32_t>(g * kTileN + row) * 16, v);

@@ -314,10 +314,12 @@ int dequantize_typed(const uint8_t* codes, int64_t codes_ld, const uint8_t* scal
                         fast_div(static_cast<uint32_t>(chunks)), gs, align == 32);
     });
   }
+  DeviceInfo dev;
+  if (const int rc = device_info(&dev)) return rc;
   const int64_t chunks = (K + 7) / 8 + 1;  // a row that starts off a boundary may touch one more
   return for_slabs(M, ((1ll << 31) - 8 * kQuantThreads) / chunks, [&](int64_t row0, int64_t rows) {
     const int64_t total = rows * chunks;
-    const bool many = total >= 2 * 148 * kQuantThreads * kDequantBatch;  // every SM (of 148) still gets two blocks
+    const bool many = total >= 2ll * dev.sm_count * kQuantThreads * kDequantBatch;  // every SM still gets two blocks
     return launch_pdl(many ? dequantize_fp4_kernel<FMT, T, kDequantBatch> : dequantize_fp4_kernel<FMT, T, 1>,
                       ceil_div64(total, kQuantThreads * (many ? kDequantBatch : 1)), kQuantThreads, stream, codes, codes_ld,
                       scales, static_cast<T*>(out), out_ld, row0, total, K, fast_div(static_cast<uint32_t>(chunks)), gs);

@@ -222,8 +222,8 @@ void check_fp4(const at::Tensor& codes, const at::Tensor& scales, int64_t K, int
 
 int64_t codes_ld(const at::Tensor& codes) { return codes.size(0) > 1 ? codes.stride(0) : codes.size(1); }
 
-// A new tensor straight from the CUDA allocator: the dispatcher's way to the same place costs a call of a few
-// microseconds a quarter of one for each.
+// A new tensor straight from the CUDA allocator: at::empty comes to the same place by way of the dispatcher (a call
+// that makes two tensors: 7.1 us of host time instead of 6.7).
 at::Tensor new_cuda(at::IntArrayRef shape, at::ScalarType dtype, const at::Device& dev) {
   return at::Tensor(at::detail::empty_cuda(shape, dtype, dev, c10::nullopt));
 }
