@@ -383,29 +383,46 @@ __device__ __forceinline__ uint32_t abs_max16(const Raw16<T>& r) {
   }
 }
 
-// silu(gate) * up in fp32: with h = exp(-|gate| / 2), gate up / (1 + h^2) for gates from 0 on, (gate h) (up h) / (1 + h^2)
-// below. The denominator is in [1, 2] and each factor h meets an operand first, so nothing overflows or vanishes on the
-// way while the result is a normal number: exp(-gate) itself is infinite from a gate of -88.7 on, where a large `up`
-// still gives one. Relative error at most 2^-20 + 2^-23 |gate|: h twice (the exponent's rounding and its constant's, 0.8
-// |gate| 2^-24 each time, and two units of ex2.approx), the reciprocal, five roundings. Gates below -174 give 0 (less than
-// 2^-116 in truth).
-//
-// Sixteen values, v[i] = silu(v[i]) * up[i], the products in pairs: 8192 x 12288 to MXFP4 72 us, one by one 75.
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2E = 1.44269504088896341f;
+
+// silu(gate) * up in fp32: gate / (1 + exp(-gate)) times up for gates from -80 on, where the denominator and its reciprocal
+// are normal numbers. Below, where 1 + exp(gate) is 1 in fp32 but exp(-gate) soon overflows, with h = exp(gate / 2) as
+// (gate h) (up h): each factor h meets an operand first, so nothing vanishes on the way while the result is a normal
+// number. Relative error at most 2^-20 + 2^-23 |gate|: the exponent's rounding and its constant's (1.25 |gate| 2^-24), two
+// units of the exponential (twice where h is), one of the reciprocal, at most four roundings. Gates below -174 give 0 (less
+// than 2^-116 in truth).
+__device__ __forceinline__ float silu_mul_any(float gate, float up) {
+  if (gate < -80.0f) {
+    const float h = exp2_approx(gate * (0.5f * kLog2E));
+    return (gate * h) * (up * h);
+  }
+  return gate * reciprocal_approx(1.0f + exp2_approx(gate * -kLog2E)) * up;
+}
+// Sixteen values, v[i] = silu(v[i]) * up[i]. Gates below -80 are rare: a thread that has none multiplies in pairs (8192 x
+// 12288 to MXFP4, L2 warm: 71.3 us, one by one 72.4).
 __device__ __forceinline__ void silu_mul16(float* v, const float* up) {
-  constexpr float kHalfLog2E = 0.72134752044448170f;
+  float least = v[0];
 #pragma unroll
-  for (int i = 0; i < 16; i += 2) {
-    float h[2], a[2], den[2];
+  for (int i = 1; i < 16; ++i) least = fminf(least, v[i]);
+  if (least >= -80.0f) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(h[j]) : "f"(fabsf(v[i + j]) * -kHalfLog2E));
-      a[j] = v[i + j] < 0.0f ? h[j] : 1.0f;
+    for (int i = 0; i < 16; i += 2) {
+      const uint64_t g = f32x2(v[i], v[i + 1]);
+      float t0, t1;
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(t0), "=f"(t1) : "l"(mul2(g, f32x2(-kLog2E, -kLog2E))));
+      const uint64_t r =
+          f32x2(reciprocal_approx(1.0f + exp2_approx(t0)), reciprocal_approx(1.0f + exp2_approx(t1)));
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(mul2(mul2(g, r), f32x2(up[i], up[i + 1]))));
     }
-    const uint64_t h2 = f32x2(h[0], h[1]), a2 = f32x2(a[0], a[1]);
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(den[0]), "=f"(den[1]) : "l"(fma2(h2, h2, f32x2(1.0f, 1.0f))));
-    const uint64_t r2 = f32x2(reciprocal_approx(den[0]), reciprocal_approx(den[1]));
-    const uint64_t y = mul2(mul2(mul2(f32x2(v[i], v[i + 1]), a2), r2), mul2(f32x2(up[i], up[i + 1]), a2));
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(v[i]), "=f"(v[i + 1]) : "l"(y));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = silu_mul_any(v[i], up[i]);
   }
 }
 
