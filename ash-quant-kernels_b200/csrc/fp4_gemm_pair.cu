@@ -13,8 +13,9 @@
 // counted on a barrier) -- no workspace, added in a fixed order.
 //
 // Bound by the tensor pipe (71 % of cycles active, the scale copies queued between the MMAs) and, in long runs, by the
-// part's power limit: 8192 x 24576 x 4096 on a B200 296-306 us in MXFP4 (5.4-5.6 PFLOP/s), 321-347 in NVFP4; 2048 x 4096
-// x 12288 34 us. Tiles of 256 x 256 because each SM then takes 68 bytes a cycle from L2 at the MMAs' nominal rate.
+// part's power limit: 8192 x 24576 x 4096 on a B200, replayed in a graph, 300-340 us in MXFP4 (4.9-5.5 PFLOP/s), 310-330 in
+// NVFP4; called in a row from Python 343-350 (4.7-4.8). 2048 x 4096 x 12288: 37 us in MXFP4, 38.5 in NVFP4. Tiles of 256 x
+// 256 because each SM then takes 68 bytes a cycle from L2 at the MMAs' nominal rate.
 //
 // TMEM (512 columns): two accumulators of 256 columns that share 128 (0..255 and 128..383), and two
 // buffers of scales. An epilogue reads the shared half first and hands it back, so the next tile's MMAs

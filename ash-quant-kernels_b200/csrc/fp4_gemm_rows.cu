@@ -16,9 +16,10 @@
 //               -> the shared memory of the CTA that adds these rows of A, counted in bytes on its barrier
 //               (st.async, or with 32 columns and more through own shared memory and bulk copies)
 //
-// Measured on a B200, launches back to back in a graph, x in fp16, MXFP4: one token 4096->6144 4.9 us, 4096->4096 4.7,
-// 4096->24576 11.7 (4.6 TB/s of weights), 12288->4096 7.6; sixteen 6.3, 5.7, 15.2, 10.9. A launch is latency from end
-// to end: 0.75 us until x is quantised, 0.2-0.3 per stage, 1 for the exchange, 0.85 to the next launch's start.
+// Measured on a B200, launches back to back in a graph, weights from HBM, x in fp16, MXFP4: one token 4096->6144 5.0 us,
+// 4096->4096 4.7, 4096->24576 12.1 (4.4 TB/s of weights), 12288->4096 8.9; sixteen 6.6, 6.0, 15.4, 10.8. A launch is
+// latency from end to end (one token 4096->6144): 0.75 us until x is quantised, 0.35 per stage, 1 for the exchange, 1 to
+// the next launch's start.
 //
 // The scales have two to eight buffers in TMEM: the copies of stage i wait for the MMAs of stage i - buffers. With
 // two, that wait and not the tensor core set the pace of narrow tiles. All waits are bounded.
@@ -467,12 +468,13 @@ struct RowsPlan {
   uint32_t off_x, off_slots, off_bar, smem;
 };
 
-// CTAs per cluster and stages in flight for `tiles` tiles of 128 weight rows (times the row blocks of A). Measured at
-// one to 128 rows on layers of 32 to 192 tiles, every cluster size and ring, launches back to back in a
-// graph. What a split saves is a CTA's serial run over its stages (0.27 us each); what it costs, beyond 1.35 CTAs
-// per SM, is the room in which the next launch's CTAs start early: 32 tiles at one row 8.0 us with one CTA
-// per cluster, 4.5 with 4 to 6, 5.8 with 7; 48 tiles 8.0, 5.0 with 4, 6.3 with 6. With more tiles than SMs a
-// split in two evens out the last wave (192 tiles: 13.4 -> 12.5 us).
+// CTAs per cluster and stages in flight for `tiles` tiles of 128 weight rows (times the row blocks of A). Measured on
+// layers of 4096 columns and 32 to 192 tiles, every cluster size, launches back to back in a graph. What a split saves is
+// a CTA's serial run over its stages; what it costs, beyond 1.35 CTAs per SM, is the room in which the next launch's CTAs
+// start early: 32 tiles at one row 7.1 us with one CTA per cluster, 4.5 with 4, 4.8 with 6, 6.0 with 7; 48 tiles 7.1, 5.1
+// with 4, 6.5 with 6. With more tiles than SMs a split in two evens out the last wave (192 tiles: 12.9 -> 12.2 us). With
+// 12288 columns and more the run weighs more than the room, which this rule does not see: 32 tiles 8.8 us with its 6 CTAs,
+// 7.5 with 7; 48 tiles 12.7 with its 4, 10.0 with 6.
 template <int FMT, int NT, bool FUSED>
 RowsPlan plan_rows(int tiles, int num_kb, int sm_count) {
   using L = RowsShape<FMT, NT, FUSED>;
@@ -601,11 +603,11 @@ int fp4_matmul_rows(const Fp4Product& p, cudaStream_t stream) {
 
 // Whether w4a4_linear quantises x inside the product: up to 32 rows, of a length whose slice fits beside the ring (an
 // eighth of it at most 48 KB), and where every 128 weight rows quantising x anew costs less than a launch for it.
-// Measured (us, fused against two launches, in a graph): up to 16 rows, at M K tiles = 6.3 million 12.8 / 15.9
-// (8 rows 4096->24576) and 11.2 / 11.7 (16 rows 12288->4096), at 12.6 million 15.3 / 16.1 (16 rows 4096->24576;
-// NVFP4 17.2 / 17.2); with the wider instruction of 32 rows 8.4 / 9.3 at 4.2 million (4096->4096), 9.8 / 9.9 at 6.3
-// million (4096->6144), 13.2 / 12.7 at 9.4 million (24 rows 12288->4096). A gated value costs two loads, an
-// exponential and a quotient more and counts three times (12288->4096: 8 rows 11.2 fused, 16 rows 16.8 against 12.5).
+// Measured (MXFP4, us, fused against two launches, in a graph): up to 16 rows, at M K tiles = 6.3 million 13.1 / 15.8 (8
+// rows 4096->24576) and 10.8 / 11.6 (16 rows 12288->4096), at 12.6 million 15.4 / 16.1 (16 rows 4096->24576; NVFP4 16.8 /
+// 17.2); with the wider instruction of 32 rows 8.9 / 9.6 at 4.2 million (4096->4096) and 10.1 / 10.1 at 6.3 million
+// (4096->6144). A gated value costs two loads, an exponential and a quotient more and counts three times (12288->4096: 4
+// rows 9.8 / 11.2, 8 rows 11.7 / 11.5).
 bool fp4_fused_ok(int M, int N, int K, bool gated) {
   const int64_t work = static_cast<int64_t>(M) * K * ceil_div(N, kTileN) * (gated ? 3 : 1);
   return M <= 16 ? K <= 32768 && work <= (1 << 24) : M <= 32 && K <= 16384 && work <= (6 << 20);

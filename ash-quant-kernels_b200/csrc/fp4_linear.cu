@@ -11,9 +11,10 @@ std::atomic<int> g_matmul_kernel{0};
 constexpr int kMaxRows = 1 << 30;  // of either operand: tile coordinates are 32-bit
 
 // Few rows go to the rows kernel, whose CTAs split K, the others to CTA pairs. Measured in graphs (MXFP4, us, rows
-// against pairs): 64 rows 8.2 / 9.4 (4096->6144), 7.9 / 9.1 (4096->4096), 10.9 / 14.9 (12288->4096), 15.2 / 17.6
-// (4096->24576); 128 rows 10.5 / 9.9, 9.0 / 9.6, 13.8 / 15.2, 17.6 / 18.7; 256 rows 10.9 / 9.9, 10.8 / 9.6,
-// 18.2 / 15.2. Between 64 and 128 rows it is the number of tiles that decides: the fewer, the finer the split of K.
+// against pairs): 64 rows 8.1 / 9.2 (4096->6144), 8.0 / 9.0 (4096->4096), 10.7 / 14.5 (12288->4096), 14.4 / 17.2
+// (4096->24576); 128 rows 9.8 / 9.7, 8.7 / 9.4, 12.7 / 14.8, 16.7 / 18.1; 256 rows 10.0 / 9.7, 10.2 / 9.5, 16.8 / 14.8,
+// 28.2 / 18.4. Between 64 and 128 rows only layers of few tiles, whose K is split finely, take the rows kernel. The wide
+// layer would gain from it too (8 % at 128 rows); where between 6144 and 24576 that begins was not measured.
 bool few_rows(int M, int N) { return M <= 64 || (M <= 128 && N <= 5120); }
 
 int fp4_matmul(const Fp4Product& p, cudaStream_t stream) {

@@ -6,7 +6,8 @@
 // half a byte of code and 1/32 or 1/16 byte of scale. At HBM speed an SM has some eleven instruction slots per
 // value, so the arithmetic is in pairs (f32x2) and offsets within a launch are 32-bit. Measured at 8192 x 12288 fp16 on
 // a B200 (L2 flushed): to MXFP4 47 us (5.4 TB/s), to NVFP4 51 us (5.0), gated 82 and 86 us (5.6, 5.3), read back 43 us
-// (6.0); 8 columns per thread and IEEE divisions took about 2.5 times as long for NVFP4.
+// (6.0); fp32 84 and 86 us (5.4, 5.3), read back 96 and 98 (4.7); 8 columns per thread and IEEE divisions took about 2.5
+// times as long for NVFP4.
 #include <algorithm>
 
 #include "fp4.cuh"
