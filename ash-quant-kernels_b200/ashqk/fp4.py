@@ -182,7 +182,7 @@ class FP4Linear(torch.nn.Module):
         assert bias is None or bias.shape == (weight.shape[0],), f"bias {tuple(bias.shape)} for {weight.shape[0]} outputs"
         self.register_buffer("codes", weight.codes)
         self.register_buffer("scales", weight.scales)
-        self.register_buffer("bias", bias)
+        self.register_buffer("bias", None if bias is None else bias.detach())
         self.out_features, self.in_features = weight.shape
         self.format, self.global_scale = weight.format, weight.global_scale
         self.input_global_scale, self.gated = input_global_scale, gated

@@ -84,3 +84,13 @@ def test_negative_block_scales_are_refused():
     nan = torch.full((3, 4), 127, dtype=torch.uint8)
     assert int(ashqk.FP4Tensor.from_rowmajor(codes, nan, "nvfp4").scales_rowmajor().min()) == 127
     ashqk.FP4Tensor.from_rowmajor(codes[:0], nan[:0], "nvfp4")
+
+
+def test_a_trained_layers_bias_brings_no_gradient():
+    """``FP4Linear(w, linear.bias)``: the layer has no gradients, so its output must not ask for one and be refused by the
+    next layer."""
+    w = ashqk.FP4Tensor(torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 1, 32, 4, 4, dtype=torch.uint8), (8, 64))
+    linear = torch.nn.Linear(64, 8)
+    layer = ashqk.FP4Linear(w, linear.bias)
+    assert not layer.bias.requires_grad and type(layer.bias) is torch.Tensor and torch.equal(layer.bias, linear.bias)
+    assert linear.bias.requires_grad

@@ -43,3 +43,16 @@ def test_input_scales_keep_activations_of_any_size(size):
     amax = xd.abs().unflatten(1, (-1, 16)).amax(2).repeat_interleave(16, 1)
     bound = torch.maximum(xd.abs() / 5, amax / 6 / 4 * (1 + 2.0**-4)) + amax / 16
     assert bool(((a - xd).abs() <= bound * (1 + 2.0**-10)).all())
+
+
+def test_layers_of_a_trained_model_in_a_row():
+    """Linear layers with their own weights and biases, converted as they are and called outside no_grad."""
+    torch.manual_seed(2)
+    up, down = (torch.nn.Linear(128, 96).cuda().half(), torch.nn.Linear(96, 64).cuda().half())
+    layers = [ashqk.FP4Linear.from_float(m.weight, m.bias, "mxfp4") for m in (up, down)]
+    x = torch.randn(5, 128, device="cuda", dtype=torch.float16)
+    h = layers[0](x)
+    y = layers[1](h)
+    assert not y.requires_grad
+    assert torch.equal(h, ashqk.w4a4_linear(x, ashqk.quantize_fp4(up.weight.detach())) + up.bias.detach())
+    assert torch.equal(y, ashqk.w4a4_linear(h, ashqk.quantize_fp4(down.weight.detach())) + down.bias.detach())
